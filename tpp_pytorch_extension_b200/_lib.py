@@ -90,6 +90,10 @@ _SIGS = {
     "tpx_diff_prefill_serves": (c_int, [c_i64, c_i64, c_f32]),
     "tpx_diff_attn": (c_int, [c_vp, c_vp]),
     "tpx_diff_status": (c_int, [c_vp, ctypes.POINTER(ctypes.c_uint)]),
+    "tpx_head_prep": (c_int, [c_vp, c_vp]),
+    "tpx_int4_read": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "tpx_int4_attention_scratch_bytes": (c_sz, [c_i64] * 5),
+    "tpx_int4_attention": (c_int, [c_vp, c_vp]),
     "tpx_qlinear": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp,
                             c_f32, c_vp, c_vp, c_sz, c_vp]),
 }
