@@ -77,6 +77,21 @@ typedef struct {
 size_t tpx_int4_attention_scratch_bytes(int64_t T, int64_t B, int64_t Nq, int64_t kv_heads, int64_t H);
 int tpx_int4_attention(const TpxInt4Attention* a, void* stream);
 
+/* Attention over whole prompts: softmax(q k^T * scale) v for the T rows q [T][Nq][H], k and v [T][Nkv][H] (ld* elements apart, heads
+ * side by side, 16-byte aligned), each within its sequence; causal: token i of a sequence sees the keys 0 .. i. Only the rows of
+ * sequences are written to out [T][Nq][H]. H 64 or 128, at most 128 query heads per key head. Values that a row does not see
+ * never reach it, infinities and NaN included. Waits inside the kernel are bounded: tpx_packed_status reads and clears the code of one that gave up. */
+typedef struct {
+  const uint16_t *q, *k, *v;
+  const int32_t* cu_seqlens;
+  uint16_t* out;
+  int64_t T, B, Nq, Nkv, H, ldq, ldk, ldv;
+  float scale;
+  int causal;
+} TpxPackedAttention;
+int tpx_packed_attention(const TpxPackedAttention* a, void* stream);
+int tpx_packed_status(void* stream, unsigned* status_host);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,8 @@ _HeadPrepStruct = _lib._struct("HeadPrepStruct", p="q k v q_norm k_norm ep pos c
                                f="eps", i="norm_is_f32")
 _Int4AttentionStruct = _lib._struct("Int4AttentionStruct", p="q cache cu_seqlens out scratch", z="scratch_bytes", l="T Nq ldq", f="scale", i="causal")
 
+_PackedAttentionStruct = _lib._struct("PackedAttentionStruct", p="q k v cu_seqlens out", l="T B Nq Nkv H ldq ldk ldv", f="scale", i="causal")
+
 
 def _check(cond, text):
     if not cond:
@@ -237,4 +239,24 @@ def attention_int4(q, cache, layer, cu_seqlens=None, causal=True, scale=None, ou
     a = _Int4AttentionStruct(q.data_ptr(), ctypes.addressof(cache.layer(layer)), cup, o.data_ptr(), sc.data_ptr(), nb, T, Nq, ldq,
                              H ** -0.5 if scale is None else scale, int(causal))
     _lib.check(L.tpx_int4_attention(ctypes.byref(a), _lib.stream()))
+    return o
+
+
+def attention_packed(q, k, v, cu_seqlens, causal=True, scale=None, out=None):
+    """Attention over whole prompts laid end to end: q bf16 [T, heads, H], k and v [T, kv_heads, H] (rows may be strided, as views of a
+    q/k/v linear's output are; H 64 or 128; up to 128 heads per key head): softmax(q k^T scale) v within each sequence, where token i
+    sees the tokens 0 .. i, or with causal=False all of them. bf16 [T, heads, H]; rows of no sequence are not written."""
+    name = "attention_packed"
+    _on_device(name, q, k, v, cu_seqlens, out)
+    _check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0,
+           f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    T, Nq, H = q.shape
+    Nkv = k.shape[1]
+    ld = _rows(name, "q", q, Nq, H), _rows(name, "k", k, Nkv, H), _rows(name, "v", v, Nkv, H)
+    _check(cu_seqlens is not None, f"{name}: cu_seqlens is needed")
+    cup = _sequences(name, cu_seqlens, None, T)
+    o = _output(name, out, (T, Nq, H), q.device)
+    a = _PackedAttentionStruct(q.data_ptr(), k.data_ptr(), v.data_ptr(), cup, o.data_ptr(), T, cu_seqlens.numel() - 1, Nq, Nkv, H, *ld,
+                               H ** -0.5 if scale is None else scale, int(causal))
+    _lib.check(_lib.lib().tpx_packed_attention(ctypes.byref(a), _lib.stream()))
     return o

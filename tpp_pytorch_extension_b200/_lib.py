@@ -94,6 +94,8 @@ _SIGS = {
     "tpx_int4_read": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "tpx_int4_attention_scratch_bytes": (c_sz, [c_i64] * 5),
     "tpx_int4_attention": (c_int, [c_vp, c_vp]),
+    "tpx_packed_attention": (c_int, [c_vp, c_vp]),
+    "tpx_packed_status": (c_int, [c_vp, ctypes.POINTER(ctypes.c_uint)]),
     "tpx_qlinear": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp,
                             c_f32, c_vp, c_vp, c_sz, c_vp]),
 }
@@ -230,7 +232,7 @@ def assert_no_kernel_error(sync=True):
         code = inst.error_code()
         if code:
             raise TpxError(f"the peer-memory all-reduce gave up waiting for rank {code - 1}")
-    for name in ("tpx_attention_tc_status", "tpx_latent_tc_status", "tpx_latent_decode_status", "tpx_diff_status"):
+    for name in ("tpx_attention_tc_status", "tpx_latent_tc_status", "tpx_latent_decode_status", "tpx_diff_status", "tpx_packed_status"):
         if _lib is not None and hasattr(_lib, name) and torch.cuda.is_available():
             st = ctypes.c_uint(0)
             check(getattr(_lib, name)(stream(), ctypes.byref(st)))
