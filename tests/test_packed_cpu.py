@@ -10,6 +10,15 @@ def P():
     return _packed_attn
 
 
+def structs():
+    from tpp_pytorch_extension_b200 import _lib
+    s = _lib._struct
+    return (s("Int4CacheStruct", p="pool table lengths", l="pages table_cols B kv_heads H"),
+            s("HeadPrepStruct", p="q k v q_norm k_norm ep pos cu_seqlens q_out k_out cache", l="T Nq Nkv H ldq ldk ldv rot max_pos ld_ep", f="eps", i="norm_is_f32"),
+            s("Int4AttentionStruct", p="q cache cu_seqlens out scratch", z="scratch_bytes", l="T Nq ldq", f="scale", i="causal"),
+            s("PackedAttentionStruct", p="q k v cu_seqlens out", l="T B Nq Nkv H ldq ldk ldv", f="scale", i="causal"))
+
+
 def lib():
     from tpp_pytorch_extension_b200 import _lib
     return _lib.lib()
@@ -20,20 +29,20 @@ A = 1 << 20  # an aligned address that no call gets as far as reading
 
 def cache(**kw):
     f = dict(pool=A, table=A, lengths=A, pages=4, table_cols=2, B=3, kv_heads=2, H=128) | kw
-    return P()._Int4CacheStruct(**f)
+    return structs()[0](**f)
 
 
 def prep(c=None, **kw):
     f = dict(q=A, k=A, v=A, q_out=A, k_out=A, T=3, Nq=4, Nkv=2, H=128, ldq=1024, ldk=1024, ldv=1024, eps=1e-6) | kw
     if c is not None:
         f["cache"] = ctypes.addressof(c)
-    a = P()._HeadPrepStruct(**f)
+    a = structs()[1](**f)
     return lib().tpx_head_prep(ctypes.byref(a), None)
 
 
 def attend(c, **kw):
     f = dict(q=A, cache=ctypes.addressof(c), out=A, scratch=A, scratch_bytes=1 << 40, T=3, Nq=4, ldq=512, scale=1.0, causal=1) | kw
-    a = P()._Int4AttentionStruct(**f)
+    a = structs()[2](**f)
     return lib().tpx_int4_attention(ctypes.byref(a), None)
 
 
@@ -111,25 +120,15 @@ def test_pages_are_handed_out_and_taken_back():
     assert sorted(p for r in c.table.tolist() for p in r if p >= 0) == [0, 1, 2, 3, 4, 5]
 
 
-def test_device_and_gradients(monkeypatch):
-    """Tensors of another device than the current one, and tensors that want a gradient."""
-    from tpp_pytorch_extension_b200 import _lib
+def packed(**kw):
+    f = dict(q=A, k=A, v=A, cu_seqlens=A, out=A, T=9, B=2, Nq=4, Nkv=2, H=128, ldq=512, ldk=256, ldv=256, scale=1.0, causal=1) | kw
+    a = structs()[3](**f)
+    return lib().tpx_packed_attention(ctypes.byref(a), None)
 
-    class T:
-        is_cuda, requires_grad, device = True, False, torch.device("cuda:1")
 
-    monkeypatch.setattr(_lib, "current_device", lambda: 0)
-    with pytest.raises(_lib.TpxError, match="current device"):
-        P()._on_device("op", T())
-    monkeypatch.setattr(_lib, "current_device", lambda: 1)
-    P()._on_device("op", T(), None, T())
-    t = T()
-    t.requires_grad = True
-    with pytest.raises(_lib.TpxError, match="no backward"):
-        P()._on_device("op", t)
-    with torch.no_grad():
-        P()._on_device("op", t)
-    t = T()
-    t.device = torch.device("cuda:0")
-    with pytest.raises(_lib.TpxError, match="cuda:1 and cuda:0"):
-        P()._on_device("op", T(), t)
+@pytest.mark.parametrize("kw,rc", [(dict(q=None), 1), (dict(v=None), 1), (dict(cu_seqlens=None), 1), (dict(out=None), 1), (dict(H=96), 2), (dict(H=256), 2), (dict(Nq=5), 1),
+                                   (dict(Nkv=0), 1), (dict(Nq=258), 2), (dict(B=0), 1), (dict(T=-1), 1), (dict(T=1 << 31), 1), (dict(k=A + 8), 1), (dict(ldv=260), 1),
+                                   (dict(T=1 << 30, Nkv=4), 1)])
+def test_packed_attention_refuses(kw, rc):
+    assert packed(**kw) == rc and lib().tpx_last_error()
+    assert packed(T=0, q=None) == 0

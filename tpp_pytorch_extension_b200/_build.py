@@ -4,7 +4,7 @@
 returns the whole library if that is up to date, else a library of only the sources that model needs.
 
 Every csrc/*.cu is compiled to an object under build/ (in parallel, only where the source or a header is newer than the
-object) and the objects are linked into libtpx_b200.so beside this file. `TPX_DEBUG=1` in the environment adds
+object) and the objects are linked into libtpx_b200.so beside this file; csrc/tpx_torch.cpp becomes the extension module _tpx_torch.so. `TPX_DEBUG=1` in the environment adds
 -DTPX_DEBUG, which compiles in the timing-experiment knobs and debug exports; the default build has none of them."""
 import concurrent.futures
 import fcntl
@@ -15,6 +15,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SO = os.path.join(HERE, "libtpx_b200.so")
+TORCH_SO = os.path.join(HERE, "_tpx_torch.so")
 OBJ_DIR = os.path.join(HERE, "build")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -53,6 +54,8 @@ def stale(so=SO, srcs=None):
 
 def build(force=False, verbose=False, so=SO, srcs=None):
     srcs = srcs or sources()
+    if so == SO:
+        build_torch(force)
     if not force and not stale(so, srcs):
         return so
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -75,6 +78,24 @@ def build(force=False, verbose=False, so=SO, srcs=None):
     subprocess.check_call([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", part] + [_obj(s) for s in srcs])
     os.replace(part, so)
     return so
+
+
+def build_torch(force=False):
+    """The extension module csrc/tpx_torch.cpp: operators on torch tensors without ctypes in between (g++, against torch's headers)."""
+    import importlib.util
+    import sysconfig
+    src = os.path.join(HERE, "csrc", "tpx_torch.cpp")
+    if not force and os.path.exists(TORCH_SO) and os.path.getmtime(TORCH_SO) >= max(os.path.getmtime(f) for f in [src] + _headers()):
+        return TORCH_SO
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    part = TORCH_SO + f".{os.getpid()}"
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f for d in inc for f in ("-isystem", d)] + ["-o", part, src, "-L" + os.path.join(torch_dir, "lib"),
+                           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], stdout=sys.stderr)
+    os.replace(part, TORCH_SO)
+    return TORCH_SO
 
 
 def ensure(architecture):

@@ -130,6 +130,27 @@ def lib():
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The extension module _tpx_torch (csrc/tpx_torch.cpp): the operators of include/tpx_packed.h on torch tensors, where the host time of a
+    ctypes call would be several times the kernel's."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib
+        L = lib()
+        try:
+            m = importlib.import_module("tpp_pytorch_extension_b200._tpx_torch")
+        except ImportError as e:
+            raise TpxError(f"the extension module _tpx_torch cannot be loaded ({e}): build it with `python -m tpp_pytorch_extension_b200._build`") from e
+        m.bind(TpxError, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value
+                           for n in ("tpx_head_prep", "tpx_int4_read", "tpx_int4_attention_scratch_bytes", "tpx_int4_attention", "tpx_packed_attention",
+                                     "tpx_last_error")))
+        _torch_ops = m
+    return _torch_ops
+
+
 class LlamaLayerStruct(ctypes.Structure):
     """TpxLlamaLayer of include/tpx_b200.h."""
     _fields_ = [(n, ctypes.c_int64) for n in ("D", "Nq", "Nkv", "H", "FF", "MP", "HR")] + \
