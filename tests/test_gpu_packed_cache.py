@@ -227,10 +227,12 @@ def check_attention(cache, q, out, old, new, cu, causal, scale, rows=None):
         kc, ks, kz, vc, vs, vz = sequence_heads(cache, b, m + n)
         x = q[at:at + n].double()
         want, w = U.attention(x, kz + kc * ks, vz + vc * vs, m, causal, scale)
-        # scores: the products of q and 16 + code and the sums of q, a rounding each for four instructions and two groups
-        size = torch.einsum("nhd,mhd->hnm", x.abs(), (kz.abs() + 48 * ks).repeat_interleave(R, 1)) * scale
-        delta = 16 * 2.0 ** -24 * size.amax(-1)                                        # [heads, n]
-        rounded = torch.einsum("hnm,mhd->nhd", w, (vs * (vc - 8).abs()).repeat_interleave(R, 1))  # weights times scales are rounded to bf16
+        # scores: q as whole numbers of 2^-19 of its row's largest value (half a step off at most, times a code of up to 15 and its
+        # scale), then some ten roundings of sums and products in fp32
+        size = torch.einsum("nhd,mhd->hnm", x.abs(), (kz.abs() + 15 * ks).repeat_interleave(R, 1)) * abs(scale)
+        steps = x.abs().amax(-1).T[..., None] * (15 * ks).repeat_interleave(R, 1).sum(-1).T[:, None] * abs(scale)
+        delta = (16 * 2.0 ** -24 * size + 2.0 ** -20 * steps).amax(-1)                 # [heads, n]
+        rounded = torch.einsum("hnm,mhd->nhd", w, (vs * (vc - 8).abs()).repeat_interleave(R, 1))  # weights times scales are rounded
         plain = torch.einsum("hnm,mhd->nhd", w, (vz.abs() + 8 * vs + vs * vc).repeat_interleave(R, 1))
         # sums in fp32 over the keys, weights off by their scores' error and that of the exponential (2^-22)
         sums = (2 * delta + 2.0 ** -20 + 2.0 ** -23 * (m + n) / 16).T[..., None] * plain

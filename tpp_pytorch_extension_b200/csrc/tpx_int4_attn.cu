@@ -2,13 +2,16 @@
 //
 //   out = softmax(scale * q K^T) V,   K[t][d] = kz + ks * kc[t][d],  V alike, with codes 0..15 and a scale and a minimum per 64 values
 //
-// Codes go to the matrix instructions as they are, scales and minima around them, so that a value costs an AND-OR (and a shift):
-//   q.K  = sum over groups of 64:  ks (q . (16 + kc)) + (kz - 16 ks) sum(q)    16 + code is a bf16 with the code as its mantissa
-//   P V  = sum over t: (p vs) (vc - 8) + p (vz + 8 vs)                          codes are centred: p vs is rounded to bf16, and that
-//                                                                              rounding should not be weighed with the range's offset
-// mma.sync m16n8k16 with the cache as the 16-row operand and the query rows ((token, group member) pairs of one key head) as its 8
-// columns: at most 8 or 16 rows share one pass over the keys (tcgen05 has no form this narrow: it would need 128 of either). Keys: M is
-// 16 tokens. Values: M is 16 of the head's dimensions, K 16 tokens; the weights get there by movmatrix.
+// The loop over the cache is bound by instructions per code, not by the matrix unit, so codes go to mma.sync as nearly as they lie there,
+// scales and minima around them (tcgen05 has no form this narrow: it would need 128 query rows or keys):
+//   q.K  = sum over groups of 64:  ks (q . kc) + kz sum(q)
+//          m16n8k32 u8 x s8: two ANDs and a shift turn eight codes into bytes. q is a 20-bit integer per value times a power of two per
+//          row, cut into three digits of 7 bits, each a column: exact products, and sums exact in 32 bits. Columns (2 r, 2 r + 1) are
+//          the upper digits of row r, so that a lane has whole scores; the accumulator starts at the bits of 1.5 * 2^23, which makes it a float.
+//   P V  = sum over t: (p vs) (vc - 8) + p (vz + 8 vs)
+//          m16n8k16 fp16: codes become fp16 by two ANDs and one HFMA2 per pair; centred, since p vs is rounded to fp16 and that should not be weighed with
+//          the range's offset. vs is taken relative to a power of two that follows the largest scale seen, which keeps p vs in fp16's range.
+// The cache is the 16-row operand: 16 tokens for keys, 16 of the head's dimensions for values. Weights get to the second product by movmatrix.
 //
 // A page of a head (4608 bytes at H = 128) is one warp's work item, fetched by cp.async into a ring of the warp's own: no barrier in the
 // loop. The (sequence, key head, row chunk) segments, each rounded up to whole quanta of GW pages (GW warps work on one segment at a
@@ -27,16 +30,30 @@ struct I4Params {
   uint16_t* out;
   const int32_t* cu;
   I4Cache c;
-  float* part;                  // [workers][2][ROWS][H + 2]: maximum, sum, output of each row
+  float* part;                   // [workers][2][ROWS][H + 2]: maximum, sum, output of each row
   unsigned long long* counters;  // [workers]
-  unsigned long long nonce;     // low 16 bits zero
+  unsigned long long nonce;      // low 16 bits zero
   int64_t ldq;
   int T, Nq, R, GW, causal;
-  float sc2;                    // scale * log2(e)
+  float sc2;                     // scale * log2(e)
 };
 
-__device__ __forceinline__ void i4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+constexpr uint32_t kI4Magic = 0x4B400000u;  // 1.5 * 2^23: a float whose low bits count whole numbers
+__device__ __forceinline__ float i4_count(int v) { return __int_as_float(v) - __uint_as_float(kI4Magic); }
+
+// d = a b + c with c the magic number in every place (first) or d
+__device__ __forceinline__ void i4_mma_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(kI4Magic));
+}
+__device__ __forceinline__ void i4_mma_u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+__device__ __forceinline__ void i4_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -50,35 +67,43 @@ __device__ __forceinline__ float i4_ex2(float x) {  // 2^-inf = 0
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t i4_pack(float lo, float hi) {
+__device__ __forceinline__ uint32_t i4_pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Codes j and j + 4 of a word as bf16 pairs: 16 + code, or code - 8
-template <int J>
-__device__ __forceinline__ uint32_t i4_plus16(uint32_t w) {
-  const uint32_t s = J == 0 ? w << 3 : w >> (4 * J - 3);
-  return (s & 0x00780078u) | 0x41804180u;
+__device__ __forceinline__ uint32_t i4_pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
-template <int J>
-__device__ __forceinline__ uint32_t i4_minus8(uint32_t w) {
-  const uint32_t v = ((w >> (4 * J)) & 0x000f000fu) | 0x43004300u;  // 128 + code
-  const uint32_t off = 0x43084308u;                                  // 136
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ float i4_pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// The codes in bits 0..3 (SHIFT 0) or 4..7 (SHIFT 4) of both halves of a word, minus 8, as fp16: 1024 + code << SHIFT is an fp16 as it stands
+template <int SHIFT>
+__device__ __forceinline__ uint32_t i4_centred(uint32_t w) {
+  const uint32_t v = (w & (0x000f000fu << SHIFT)) | 0x64006400u;
+  uint32_t r;
+  if (SHIFT == 0) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0xe408e408u));                        // -1032
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0x2c002c00u), "r"(0xd480d480u));              // / 16, - 72
+  return r;
 }
 __device__ __forceinline__ void i4_cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void i4_lds(uint32_t a, uint32_t (&v)[4]) {
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+template <int N>
+__device__ __forceinline__ void i4_lds(const unsigned char* a, uint32_t (&v)[N]) {  // N words, 4 N-byte aligned
+  if (N == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(a);
+    v[0] = x.x; v[1 % N] = x.y; v[2 % N] = x.z; v[3 % N] = x.w;
+  } else if (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(a);
+    v[0] = x.x; v[1 % N] = x.y;
+  } else {
+    v[0] = *reinterpret_cast<const uint32_t*>(a);
+  }
 }
-__device__ __forceinline__ void i4_lds(uint32_t a, uint32_t (&v)[2]) {
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
-}
-__device__ __forceinline__ void i4_lds(uint32_t a, uint32_t (&v)[1]) { asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(a)); }
 
-// Work of one sequence
+// Work of one sequence. A quantum is GW pages, one per warp of a group; a piece is what is never cut between groups: one quantum, or
+// four where there is too little work for all groups anyway (two more quanta in a row cost less than adding up partial results).
+constexpr int kI4Piece = 4;
 struct I4Seq {
   int n, keys, quanta, chunks;  // tokens of the call, keys, quanta of a segment, row chunks
 };
@@ -97,111 +122,110 @@ __device__ __forceinline__ I4Seq i4_seq(const I4Params& p, int b, int rows) {
   return s;
 }
 
-template <int H, int NT>
+// RT: query rows per lane, 4 RT in a chunk
+template <int H, int RT>
 struct I4Cfg {
-  static constexpr int ROWS = 8 * NT;
+  static constexpr int ROWS = 4 * RT;
   static constexpr int STAGES = 2;
-  static constexpr int WARPS = NT == 1 ? kI4Warps : kI4Warps / 2;
-  static constexpr int PITCH = H + 4;                     // floats of a row in the merge buffer
+  static constexpr int WARPS = RT < 4 ? kI4Warps : kI4Warps / 2;
+  static constexpr int TILES = RT + (RT + 1) / 2;          // n-tiles of q digits: upper two of 4 rows each, lowest of 8
+  static constexpr int PITCH = H + 4;                      // floats of a row in the merge buffer
   static constexpr int MERGE = (ROWS * PITCH + 2 * ROWS) * 4;
-  static constexpr int WARP_BYTES = STAGES * I4<H>::BYTES + MERGE;
+  static constexpr int QBUF = TILES * (H / 32) * 256 + ROWS * 16;  // digits, then (scale, sums of q) of each row: a group's, over its first warp's merge buffer
+  static constexpr int WARP_BYTES = STAGES * I4<H>::BYTES + (MERGE > QBUF ? MERGE : QBUF);
   static constexpr int SMEM = WARPS * WARP_BYTES;
 };
 
-template <int H, int NT>
-__global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(const I4Params p) {
-  using C = I4Cfg<H, NT>;
+template <int H, int RT>
+__global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(const I4Params p) {
+  using C = I4Cfg<H, RT>;
   using L = I4<H>;
-  constexpr int ROWS = C::ROWS, G = L::G, WPK = H / 32;  // WPK: words of a lane per key row
+  constexpr int ROWS = C::ROWS, G = L::G, WPK = H / 32, VT = (RT + 1) / 2;  // WPK: words of a lane per key row; VT: n-tiles of weights
   extern __shared__ __align__(16) unsigned char i4_smem[];
-  __shared__ long long scan[C::WARPS + 1];
-  __shared__ int start_b;
-  __shared__ long long start_off;
+  __shared__ int scan[2][C::WARPS], start_off[C::WARPS];
+  __shared__ int start_b[C::WARPS];
   pdl_trigger();
   pdl_wait();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int GW = p.GW, grp = warp / GW, w = warp % GW, gtid = threadIdx.x - grp * GW * 32;
-  const long long workers = (long long)gridDim.x * (C::WARPS / GW), me = (long long)blockIdx.x * (C::WARPS / GW) + grp;
+  const int workers = (int)gridDim.x * (C::WARPS / GW), me = (int)blockIdx.x * (C::WARPS / GW) + grp;
   auto group_sync = [&]() {
     if (GW == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(GW * 32) : "memory");
   };
 
-  // ---- the quanta of all segments, and this group's share of them
-  long long total;
+  // ---- the pieces of all segments, and this group's share of them
   const int per_thread = (p.c.B + blockDim.x - 1) / blockDim.x;
   const int b_lo = min((int)threadIdx.x * per_thread, p.c.B), b_hi = min(b_lo + per_thread, p.c.B);
-  long long mine = 0;
+  int mine[2] = {0, 0};  // in pieces of one quantum, of four
   for (int b = b_lo; b < b_hi; b++) {
     const I4Seq s = i4_seq(p, b, ROWS);
-    mine += (long long)s.quanta * s.chunks * p.c.Nkv;
+    const int segments = (int)s.chunks * p.c.Nkv;
+    mine[0] += segments * s.quanta;
+    mine[1] += segments * ((s.quanta + kI4Piece - 1) / kI4Piece);
   }
-  long long incl = mine;
+  int incl[2] = {mine[0], mine[1]};
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int v = __shfl_up_sync(0xffffffffu, incl[k], o);
+      if (lane >= o) incl[k] += v;
+    }
   }
-  if (lane == 31) scan[warp + 1] = incl;
-  if (threadIdx.x == 0) scan[0] = 0;
+  if (lane == 31) {
+    scan[0][warp] = incl[0];
+    scan[1][warp] = incl[1];
+  }
   __syncthreads();
-  long long before = 0;
-  total = 0;
+  int before[2] = {0, 0}, totals[2] = {0, 0};
   for (int i = 0; i < C::WARPS; i++) {
-    if (i < warp) before += scan[i + 1];
-    total += scan[i + 1];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      if (i < warp) before[k] += scan[k][i];
+      totals[k] += scan[k][i];
+    }
   }
-  const long long excl = before + incl - mine;
-  const long long per = (total + workers - 1) / workers;
-  // where each group starts: the thread whose sequences hold that quantum says so, one group after the other
-  long long q0 = 0, q1 = 0, at = 0;
-  int b0 = 0;
+  const bool few = totals[0] <= kI4Piece * workers;
+  const int PIECE = few ? kI4Piece : 1;
+  const int total = few ? totals[1] : totals[0], held_here = few ? mine[1] : mine[0], excl = few ? before[1] + incl[1] - mine[1] : before[0] + incl[0] - mine[0];
+  const int per = (total + workers - 1) / workers;
+  // where each group starts: the thread whose sequences hold that piece says so
   for (int k = 0; k < C::WARPS / GW; k++) {
-    const long long s0 = ((long long)blockIdx.x * (C::WARPS / GW) + k) * per, s1 = min(s0 + per, total);
-    __syncthreads();
-    if (s0 < s1 && excl <= s0 && s0 < excl + mine) {
-      long long acc = excl;
+    const int s0 = ((int)blockIdx.x * (C::WARPS / GW) + k) * per;
+    if (s0 < total && excl <= s0 && s0 < excl + held_here) {
+      int acc = excl;
       for (int b = b_lo; b < b_hi; b++) {
         const I4Seq s = i4_seq(p, b, ROWS);
-        const long long n = (long long)s.quanta * s.chunks * p.c.Nkv;
+        const int n = (int)((s.quanta + PIECE - 1) / PIECE) * s.chunks * p.c.Nkv;
         if (s0 < acc + n) {
-          start_b = b;
-          start_off = s0 - acc;
+          start_b[k] = b;
+          start_off[k] = s0 - acc;
           break;
         }
         acc += n;
       }
     }
-    __syncthreads();
-    if (k == grp) {
-      q0 = s0;
-      q1 = s1;
-      b0 = start_b;
-      at = start_off;
-    }
   }
+  __syncthreads();
+  const int q0 = me * per, q1 = min(q0 + per, total);
   if (q0 >= q1) return;  // whole groups leave; what follows synchronises groups only
 
   // ---- iterators over the quanta of the share
   struct Iter {
     int b, n, chunk, qi;  // sequence, key head, row chunk, quantum of the segment
+    int piece;      // of all pieces
     I4Seq s;
   };
-  auto begin = [&]() {
-    Iter i;
-    i.b = b0;
-    i.s = i4_seq(p, b0, ROWS);
-    const long long per_head = (long long)i.s.quanta * i.s.chunks;
-    i.n = (int)(at / per_head);
-    const int r = (int)(at % per_head);
-    i.chunk = r / i.s.quanta;
-    i.qi = r % i.s.quanta;
-    return i;
-  };
-  auto advance = [&](Iter& i) {  // only while quanta are left
-    if (++i.qi < i.s.quanta) return;
+  auto advance = [&](Iter& i) {
+    if (++i.qi < i.s.quanta) {
+      if (i.qi % PIECE == 0) i.piece++;
+      return;
+    }
+    i.piece++;
     i.qi = 0;
+    if (i.piece >= q1) return;
     if (++i.chunk < i.s.chunks) return;
     i.chunk = 0;
     if (++i.n < p.c.Nkv) return;
@@ -212,107 +236,155 @@ __global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(
       i.s = i4_seq(p, i.b, ROWS);
     } while (i.s.quanta * i.s.chunks == 0);
   };
+  Iter now;
+  {
+    now.b = start_b[grp];
+    now.s = i4_seq(p, now.b, ROWS);
+    const int pieces = (now.s.quanta + PIECE - 1) / PIECE;
+    const int at = start_off[grp], per_head = (int)pieces * now.s.chunks;
+    now.n = (int)(at / per_head);
+    const int r = (int)(at % per_head);
+    now.chunk = r / pieces;
+    now.qi = r % pieces * PIECE;
+    now.piece = q0;
+  }
 
   unsigned char* base = i4_smem + warp * C::WARP_BYTES;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(base);
   float* merge = reinterpret_cast<float*>(base + C::STAGES * L::BYTES);
   unsigned char* group_base = i4_smem + grp * GW * C::WARP_BYTES + C::STAGES * L::BYTES;
 
-  // Fetches this warp's page of the iterator's quantum; the keys that it holds (0: no page)
-  auto fetch = [&](const Iter& i, int stage) -> int {
+  // The table's entry for this warp's page of an iterator's quantum, asked for one round before it is needed (-1: no page)
+  auto entry = [&](const Iter& i) -> int {
     const int pg = i.qi * GW + w;
-    int live = i.s.keys - pg * kI4Page;
-    if (live > 0) {
-      const int page = p.c.table[(int64_t)i.b * p.c.cols + pg];
-      if (page >= 0 && page < p.c.pages) {
-        const uint8_t* src = p.c.pool + ((int64_t)page * p.c.Nkv + i.n) * L::BYTES + lane * 16;
-        const uint32_t dst = ring + stage * L::BYTES + lane * 16;
+    return i.piece < q1 && pg * kI4Page < i.s.keys ? p.c.table[(int64_t)i.b * p.c.cols + pg] : -1;
+  };
+  // Fetches that page; the keys that it holds (0: no page)
+  auto fetch = [&](const Iter& i, int page, int stage) -> int {
+    if (page < 0 || page >= p.c.pages) return 0;
+    const uint8_t* src = p.c.pool + ((int64_t)page * p.c.Nkv + i.n) * L::BYTES + lane * 16;
+    const uint32_t dst = ring + stage * L::BYTES + lane * 16;
 #pragma unroll
-        for (int k = 0; k < L::BYTES / 512; k++) i4_cp16(dst + k * 512, src + k * 512);
-        if (L::BYTES % 512 && lane < L::BYTES % 512 / 16) i4_cp16(dst + L::BYTES / 512 * 512, src + L::BYTES / 512 * 512);
-      } else {
-        live = 0;
-      }
-    }
-    return min(max(live, 0), kI4Page);
+    for (int k = 0; k < L::BYTES / 512; k++) i4_cp16(dst + k * 512, src + k * 512);
+    if (L::BYTES % 512 && lane < L::BYTES % 512 / 16) i4_cp16(dst + L::BYTES / 512 * 512, src + L::BYTES / 512 * 512);
+    return min(i.s.keys - (i.qi * GW + w) * kI4Page, kI4Page);
   };
 
-  Iter ahead = begin(), now = ahead;
-  long long qa = q0;
+  Iter ahead = now;
+  int ahead_page = entry(ahead);
   int held[C::STAGES];
-#pragma unroll
-  for (int s = 0; s < C::STAGES; s++) {
-    held[s] = 0;
-    if (qa < q1) {
-      held[s] = fetch(ahead, s);
-      if (++qa < q1) advance(ahead);
-    }
+  static_assert(C::STAGES == 2, "the first two pages");
+  {
+    const Iter first = ahead;
+    const int first_page = ahead_page;
+    advance(ahead);
+    ahead_page = entry(ahead);  // both entries are asked for before either is used
+    held[0] = fetch(first, first_page, 0);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    held[1] = fetch(ahead, ahead_page, 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (ahead.piece < q1) advance(ahead);
+    ahead_page = entry(ahead);
   }
 
-  uint32_t qf[NT][WPK][4];
-  float qs[NT][G][2];                        // sums of q over each group, rows 2t and 2t + 1
-  float acc[NT][G][4][4], zacc[NT][G][2], m_run[NT][2], l_run[NT][2];
-  int klim[NT][2], klim_min = 0;
+  uint2 qf[C::TILES][WPK];
+  float qsc[RT], qs[RT][G];                // per row: 2^-k scale log2(e), and sums of q times scale log2(e)
+  float acc[VT][G][4][4], zacc[RT][G], m_run[RT], l_run[RT];
+  int klim[RT], klim_min = 0, vexp = -126;  // values are kept in units of 2^vexp
   bool fresh = true;
+  const int kr = (g >> 1) + 4 * (g & 1);   // row g of a 16-row tile is key kr of its first 8, row g + 8 of its last 8
 
-  for (long long qc = q0; qc < q1; qc++) {
-    const int stage = (int)((qc - q0) % C::STAGES);
-    if (fresh) {  // a new segment: its query rows
+  for (int stage = 0; now.piece < q1; stage = stage + 1 == C::STAGES ? 0 : stage + 1) {
+    if (fresh) {  // a new segment: its query rows, as digits, by the group together
       fresh = false;
       const int tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
-      const long long cap = (long long)p.c.cols * kI4Page, first = max(p.c.lengths[now.b], 0);
+      constexpr int LR = H / 8;  // lanes per row
+      uint2* frag = reinterpret_cast<uint2*>(group_base);
+      float4* info = reinterpret_cast<float4*>(group_base + C::TILES * WPK * 256);
+      for (int r0 = w * (32 / LR); r0 < ROWS; r0 += GW * (32 / LR)) {
+        const int r = r0 + lane / LR, u = lane % LR, row = now.chunk * ROWS + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < ROWS && row < now.s.n * p.R)
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(tok0 + row / p.R) * p.ldq + (int64_t)(now.n * p.R + row % p.R) * H + 8 * u);
+        const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+        float x[8], top = 0.0f, sum = 0.0f, bad = 0.0f;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const int row = now.chunk * ROWS + nt * 8 + g;
-        const bool live = row < now.s.n * p.R;
-        const uint16_t* src = p.q + (int64_t)(tok0 + (live ? row / p.R : 0)) * p.ldq + (int64_t)(now.n * p.R + (live ? row % p.R : 0)) * H;
-        float sum[G];
-#pragma unroll
-        for (int h = 0; h < G; h++) sum[h] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < WPK; i++) {
-          const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * t) : make_uint4(0, 0, 0, 0);
-          qf[nt][i][0] = __byte_perm(v.x, v.z, 0x5410);  // values 0 and 4 of the lane's 8
-          qf[nt][i][1] = __byte_perm(v.x, v.z, 0x7632);  // 1 and 5
-          qf[nt][i][2] = __byte_perm(v.y, v.w, 0x5410);
-          qf[nt][i][3] = __byte_perm(v.y, v.w, 0x7632);
-#pragma unroll
-          for (int j = 0; j < 4; j++) sum[i / 2] += __uint_as_float(qf[nt][i][j] << 16) + __uint_as_float(qf[nt][i][j] & 0xffff0000u);
+        for (int i = 0; i < 4; i++) {
+          x[2 * i] = __uint_as_float(vw[i] << 16);
+          x[2 * i + 1] = __uint_as_float(vw[i] & 0xffff0000u);
         }
 #pragma unroll
-        for (int h = 0; h < G; h++) {
-          float s = sum[h];
-          s += __shfl_xor_sync(0xffffffffu, s, 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          qs[nt][h][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-          qs[nt][h][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-          zacc[nt][h][0] = zacc[nt][h][1] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[nt][h][i][0] = acc[nt][h][i][1] = acc[nt][h][i][2] = acc[nt][h][i][3] = 0.0f;
+        for (int i = 0; i < 8; i++) {
+          top = fmaxf(top, fabsf(x[i]));
+          sum += x[i];
+          bad = fmaf(x[i], 0.0f, bad);  // a NaN where any value is not finite
         }
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          // rows behind the last are computed with the last token's keys and not written
-          const int tok = min((now.chunk * ROWS + nt * 8 + 2 * t + e) / p.R, now.s.n - 1);
-          klim[nt][e] = p.causal ? (int)min(cap, first + tok + 1) : now.s.keys;
-          m_run[nt][e] = -INFINITY;
-          l_run[nt][e] = 0.0f;
+        for (int o = LR / 2; o > 0; o >>= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          bad += __shfl_xor_sync(0xffffffffu, bad, o);
+          if (o < 8) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // within a group of 64
+        }
+        const float other = __shfl_xor_sync(0xffffffffu, sum, LR / 2);
+        // top * 2^k in [2^19, 2^20): 20 bits
+        const int k = min(19 - ((int)((__float_as_uint(top) >> 23) & 255) - 127), 120);
+        const float up = i4_pow2(k);
+        uint32_t d[3][2] = {};  // digits: bytes of the even and of the odd values
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int Q = (int)(__float_as_uint(fmaf(x[i], up, __uint_as_float(kI4Magic))) - kI4Magic);
+          const int hi = (Q + 8192) >> 14, rem = Q - (hi << 14), mid = (rem + 64) >> 7, lo = rem - (mid << 7);
+          d[0][i & 1] |= (uint32_t)(hi & 255) << (8 * (i >> 1));
+          d[1][i & 1] |= (uint32_t)(mid & 255) << (8 * (i >> 1));
+          d[2][i & 1] |= (uint32_t)(lo & 255) << (8 * (i >> 1));
+        }
+        if (r < ROWS) {
+          const int tile = r / 4, col = 2 * (r % 4), i = u / 4, tt = u % 4;
+          frag[(tile * WPK + i) * 32 + col * 4 + tt] = make_uint2(d[0][0], d[0][1]);
+          frag[(tile * WPK + i) * 32 + (col + 1) * 4 + tt] = make_uint2(d[1][0], d[1][1]);
+          frag[((RT + tile / 2) * WPK + i) * 32 + (col + (tile & 1)) * 4 + tt] = make_uint2(d[2][0], d[2][1]);
+          if (u == 0) info[r] = make_float4(i4_pow2(-k) * p.sc2 + bad, sum * p.sc2, G == 2 ? other * p.sc2 : 0.0f, 0.0f);
         }
       }
+      group_sync();
+#pragma unroll
+      for (int i = 0; i < C::TILES; i++)
+#pragma unroll
+        for (int k = 0; k < WPK; k++) qf[i][k] = frag[(i * WPK + k) * 32 + lane];
+      const long long cap = (long long)p.c.cols * kI4Page, first = max(p.c.lengths[now.b], 0);
+#pragma unroll
+      for (int j = 0; j < RT; j++) {
+        const float4 f = info[4 * j + t];
+        qsc[j] = f.x;
+        qs[j][0] = f.y;
+        if (G == 2) qs[j][G - 1] = f.z;
+        // rows behind the last are computed with the last token's keys and not written
+        const int tok = min((now.chunk * ROWS + 4 * j + t) / p.R, now.s.n - 1);
+        klim[j] = p.causal ? (int)min(cap, first + tok + 1) : now.s.keys;
+        m_run[j] = -INFINITY;
+        l_run[j] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < G; h++) zacc[j][h] = 0.0f;
+      }
       klim_min = p.causal ? (int)min(cap, first + now.chunk * ROWS / p.R + 1) : now.s.keys;
+      vexp = -126;
+#pragma unroll
+      for (int v = 0; v < VT; v++)
+#pragma unroll
+        for (int h = 0; h < G; h++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[v][h][i][0] = acc[v][h][i][1] = acc[v][h][i][2] = acc[v][h][i][3] = 0.0f;
     }
 
     asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
     __syncwarp();
     const int have = held[0];
     if (have > 0) {
-      const uint32_t st = ring + stage * L::BYTES;
+      const unsigned char* st = base + stage * L::BYTES;
       const int key0 = (now.qi * GW + w) * kI4Page;
-      // ---- scores of 32 keys: rows of two m16 tiles; row i of a tile is key i / 2 + 4 (i % 2) of its first 8, then of its last 8
-      float x[NT][2][4];
+      // ---- scores of 32 keys, in units of log2(e): x[row][tile of 16 keys][its first or last 8]
+      float x[RT][2][2];
       uint32_t vparam[2][2][G];
-      const int kr = (g >> 1) + 4 * (g & 1);
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         uint32_t kw[2][WPK], kp[2][G];
@@ -324,103 +396,139 @@ __global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(
           i4_lds(st + L::VP + key * (G * 4), vparam[m][r]);
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) x[nt][m][0] = x[nt][m][1] = x[nt][m][2] = x[nt][m][3] = 0.0f;
-#pragma unroll
         for (int h = 0; h < G; h++) {
-          float d[NT][4];
+          int d[C::TILES][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.0f;
+          for (int i = 0; i < 2; i++) {
+            const uint32_t a = kw[0][2 * h + i], b = kw[1][2 * h + i];
+            const uint32_t a0 = a & 0x0f0f0f0fu, a1 = b & 0x0f0f0f0fu, a2 = (a >> 4) & 0x0f0f0f0fu, a3 = (b >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-          for (int i = 2 * h; i < 2 * h + 2; i++) {
-            const uint32_t a = kw[0][i], b = kw[1][i];
-            const uint32_t f[8] = {i4_plus16<0>(a), i4_plus16<0>(b), i4_plus16<1>(a), i4_plus16<1>(b),
-                                   i4_plus16<2>(a), i4_plus16<2>(b), i4_plus16<3>(a), i4_plus16<3>(b)};
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              i4_mma(d[nt], f[0], f[1], f[2], f[3], qf[nt][i][0], qf[nt][i][1]);
-              i4_mma(d[nt], f[4], f[5], f[6], f[7], qf[nt][i][2], qf[nt][i][3]);
+            for (int n = 0; n < C::TILES; n++) {
+              if (i == 0) i4_mma_first(d[n], a0, a1, a2, a3, qf[n][2 * h]);
+              else i4_mma_u8(d[n], a0, a1, a2, a3, qf[n][2 * h + 1]);
             }
           }
 #pragma unroll
           for (int r = 0; r < 2; r++) {
-            const float s = __uint_as_float(kp[r][h] << 16), z = fmaf(-16.0f, s, __uint_as_float(kp[r][h] & 0xffff0000u));
+            const float s = __uint_as_float(kp[r][h] << 16), z = __uint_as_float(kp[r][h] & 0xffff0000u);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-              for (int e = 0; e < 2; e++) x[nt][m][2 * r + e] = fmaf(s, d[nt][2 * r + e], fmaf(z, qs[nt][h][e], x[nt][m][2 * r + e]));
+            for (int j = 0; j < RT; j++) {
+              const float f = fmaf(fmaf(i4_count(d[j][2 * r]), 128.0f, i4_count(d[j][2 * r + 1])), 128.0f, i4_count(d[RT + j / 2][2 * r + (j & 1)]));
+              x[j][m][r] = fmaf(s * qsc[j], f, h == 0 ? z * qs[j][0] : fmaf(z, qs[j][h], x[j][m][r]));
+            }
           }
         }
       }
-      const bool edge = key0 + kI4Page > klim_min || have < kI4Page;
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+      bool odd = false;  // a key that some row sees and another does not has no finite value
+      if (key0 + kI4Page > klim_min || have < kI4Page) {
 #pragma unroll
         for (int m = 0; m < 2; m++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            x[nt][m][i] *= p.sc2;
-            if (edge && key0 + 16 * m + 8 * (i >> 1) + kr >= klim[nt][i & 1]) x[nt][m][i] = -INFINITY;
-          }
-      // ---- the running maximum is a reference that has to follow only when a score passes it by 2^8
-      bool pass = false;
-      float top[NT][2];
+          for (int r = 0; r < 2; r++) {
+            const int key = 16 * m + 8 * r + kr;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          top[nt][e] = fmaxf(fmaxf(x[nt][0][e], x[nt][0][2 + e]), fmaxf(x[nt][1][e], x[nt][1][2 + e]));
-          pass |= top[nt][e] > m_run[nt][e] + 8.0f;
-        }
-      if (__any_sync(0xffffffffu, pass)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float v = top[nt][e];
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            const float m_new = fmaxf(m_run[nt][e], v);
-            const float alpha = m_new == m_run[nt][e] ? 1.0f : i4_ex2(m_run[nt][e] - m_new);
-            m_run[nt][e] = m_new;
-            l_run[nt][e] *= alpha;
+            for (int j = 0; j < RT; j++)
+              if (key0 + key >= klim[j]) x[j][m][r] = -INFINITY;
 #pragma unroll
             for (int h = 0; h < G; h++) {
-              zacc[nt][h][e] *= alpha;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                acc[nt][h][i][e] *= alpha;
-                acc[nt][h][i][2 + e] *= alpha;
-              }
+              if (key >= have) vparam[m][r][h] = 0;  // places behind the last token may hold anything
+              odd |= (vparam[m][r][h] & 0x7f800000u) == 0x7f800000u;
             }
           }
+        odd = __any_sync(0xffffffffu, odd);
       }
+      // ---- the running maximum is a reference that has to follow only when a score passes it by 2^8, the unit of the values one
+      // that follows when a scale passes it by 2^7: weights times scales then stay below 2^15
+      bool pass = false;
+      float top[RT];
+      uint32_t smax = 0;  // low half: the largest scale's bits
+#pragma unroll
+      for (int j = 0; j < RT; j++) {
+        top[j] = fmaxf(fmaxf(x[j][0][0], x[j][0][1]), fmaxf(x[j][1][0], x[j][1][1]));
+        pass |= top[j] > m_run[j] + 8.0f;
+      }
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+          for (int h = 0; h < G; h++) smax = __vmaxu2(smax, vparam[m][r][h]);
+      pass |= (int)((smax >> 7) & 255) > vexp + 127 + 6;
+      if (__any_sync(0xffffffffu, pass)) {
+        int e = 0;
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int h = 0; h < G; h++) {
+              const int b = (vparam[m][r][h] >> 7) & 255;
+              if (b != 255) e = max(e, b);  // not a NaN's
+            }
+        e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e) - 127;
+        // the largest scale is below 2^(e + 1): with e <= vexp + 6 it stays, else it becomes 2^6 .. 2^7 units
+        const int v_new = e > vexp + 6 ? max(e - 6, -126) : vexp;
+        const float down = v_new - vexp > 126 ? 0.0f : i4_pow2(vexp - v_new);
+        vexp = v_new;
+        float alpha[RT];
+#pragma unroll
+        for (int j = 0; j < RT; j++) {
+          float v = top[j];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+          const float m_new = fmaxf(m_run[j], v);
+          alpha[j] = m_new == m_run[j] ? 1.0f : i4_ex2(m_run[j] - m_new);
+          m_run[j] = m_new;
+          l_run[j] *= alpha[j];
+#pragma unroll
+          for (int h = 0; h < G; h++) zacc[j][h] *= alpha[j];
+        }
+#pragma unroll
+        for (int v = 0; v < VT; v++)
+#pragma unroll
+          for (int h = 0; h < G; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+              for (int k = 0; k < 4; k++) acc[v][h][i][k] *= (RT == 1 ? alpha[0] : alpha[2 * v + (k & 1)]) * down;
+      }
+      float ref[RT];
+#pragma unroll
+      for (int j = 0; j < RT; j++) ref[j] = m_run[j] == -INFINITY ? 0.0f : m_run[j];
+      const float unit = i4_pow2(min(-vexp, 126));
       // ---- weights, and values of 16 keys at a time
 #pragma unroll
       for (int m = 0; m < 2; m++) {
-        uint32_t pb[NT][G][2];
+        uint32_t pb[VT][RT == 1 ? 1 : G][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          float e4[4];
+        for (int r = 0; r < 2; r++) {
+          float e[RT];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float ref = m_run[nt][i & 1];
-            e4[i] = ref == -INFINITY ? 0.0f : i4_ex2(x[nt][m][i] - ref);
-            l_run[nt][i & 1] += e4[i];
+          for (int j = 0; j < RT; j++) {
+            e[j] = i4_ex2(x[j][m][r] - ref[j]);
+            l_run[j] += e[j];
           }
+          float ps[RT][G];  // weight times scale
 #pragma unroll
           for (int h = 0; h < G; h++) {
+            const float s = __uint_as_float(vparam[m][r][h] << 16), z = fmaf(8.0f, s, __uint_as_float(vparam[m][r][h] & 0xffff0000u)), su = s * unit;
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-              const float s = __uint_as_float(vparam[m][r][h] << 16), z = fmaf(8.0f, s, __uint_as_float(vparam[m][r][h] & 0xffff0000u));
-              float a = e4[2 * r] * s, b = e4[2 * r + 1] * s, za = e4[2 * r] * z, zb = e4[2 * r + 1] * z;
-              if (edge) {  // what a row does not see leaves it alone, whatever it is
-                if (x[nt][m][2 * r] == -INFINITY) a = za = 0.0f;
-                if (x[nt][m][2 * r + 1] == -INFINITY) b = zb = 0.0f;
+            for (int j = 0; j < RT; j++) {
+              if (odd && x[j][m][r] == -INFINITY) {  // what a row does not see leaves it alone
+                ps[j][h] = 0.0f;
+              } else {
+                ps[j][h] = e[j] * su;
+                zacc[j][h] = fmaf(e[j], z, zacc[j][h]);
               }
-              zacc[nt][h][0] += za;
-              zacc[nt][h][1] += zb;
-              pb[nt][h][r] = i4_transpose(i4_pack(a, b));
             }
+          }
+          if (RT == 1) {  // columns (row t, group): both groups' products share the operand
+            pb[0][0][r] = i4_transpose(i4_pack_f16(ps[0][0], G == 2 ? ps[0][G - 1] : 0.0f));
+          } else {        // columns (row t, row t + 4) of each group
+#pragma unroll
+            for (int v = 0; v < VT; v++)
+#pragma unroll
+              for (int h = 0; h < G; h++) pb[v][RT == 1 ? 0 : h][r] = i4_transpose(i4_pack_f16(ps[RT == 1 ? 0 : 2 * v][h], ps[RT == 1 ? 0 : 2 * v + 1][h]));
           }
         }
         uint32_t va[2 * G], vb[2 * G];  // [key t, key t + 4][group] of the first and the last 8 keys
@@ -428,71 +536,84 @@ __global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(
         i4_lds(st + L::VC + (((2 * m + 1) * 8 + g) * 4 + t) * (8 * G), vb);
 #pragma unroll
         for (int h = 0; h < G; h++) {
-          const uint32_t xa = __byte_perm(va[h], va[G + h], 0x5410), ya = __byte_perm(va[h], va[G + h], 0x7632);
-          const uint32_t xb = __byte_perm(vb[h], vb[G + h], 0x5410), yb = __byte_perm(vb[h], vb[G + h], 0x7632);
-#define TPX_I4_V(I)                                                                                                    \
-  {                                                                                                                    \
-    const uint32_t f0 = i4_minus8<I>(xa), f1 = i4_minus8<I>(ya), f2 = i4_minus8<I>(xb), f3 = i4_minus8<I>(yb);         \
-    _Pragma("unroll") for (int nt = 0; nt < NT; nt++) i4_mma(acc[nt][h][I], f0, f1, f2, f3, pb[nt][h][0], pb[nt][h][1]); \
-  }
-          TPX_I4_V(0) TPX_I4_V(1) TPX_I4_V(2) TPX_I4_V(3)
-#undef TPX_I4_V
+          // low halves: dimensions 64 h + 8 g + 0..3 of the keys t and t + 4, high halves: + 4..7
+          uint32_t xa = __byte_perm(va[h], va[G + h], 0x5410), ya = __byte_perm(va[h], va[G + h], 0x7632);
+          uint32_t xb = __byte_perm(vb[h], vb[G + h], 0x5410), yb = __byte_perm(vb[h], vb[G + h], 0x7632);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const uint32_t f0 = i4_centred<0>(xa), f1 = i4_centred<0>(ya), f2 = i4_centred<0>(xb), f3 = i4_centred<0>(yb);
+            const uint32_t f4 = i4_centred<4>(xa), f5 = i4_centred<4>(ya), f6 = i4_centred<4>(xb), f7 = i4_centred<4>(yb);
+#pragma unroll
+            for (int v = 0; v < VT; v++) {
+              const uint32_t(&b)[2] = pb[v][RT == 1 ? 0 : h];
+              i4_mma_f16(acc[v][h][i], f0, f1, f2, f3, b[0], b[1]);
+              i4_mma_f16(acc[v][h][i + 1], f4, f5, f6, f7, b[0], b[1]);
+            }
+            xa >>= 8;
+            ya >>= 8;
+            xb >>= 8;
+            yb >>= 8;
+          }
         }
       }
     }
     __syncwarp();  // the stage has been read by every lane
 #pragma unroll
     for (int s = 0; s + 1 < C::STAGES; s++) held[s] = held[s + 1];
-    held[C::STAGES - 1] = 0;
-    if (qa < q1) {
-      held[C::STAGES - 1] = fetch(ahead, stage);
-      if (++qa < q1) advance(ahead);
-    }
+    held[C::STAGES - 1] = fetch(ahead, ahead_page, stage);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    if (ahead.piece < q1) advance(ahead);
+    ahead_page = entry(ahead);
 
     const bool last_of_segment = now.qi + 1 == now.s.quanta;
-    if (last_of_segment || qc + 1 == q1) {
+    if (last_of_segment || (now.piece + 1 == q1 && (now.qi + 1) % PIECE == 0)) {
       // ---- this group's part of the segment: rows of (maximum, sum, output), merged over its warps
+      const int rows = min(ROWS, now.s.n * p.R - now.chunk * ROWS);
       float* ml = merge + ROWS * C::PITCH;
+      const float up = i4_pow2(min(vexp, 126));
+      if (GW > 1) group_sync();  // the first warp's buffer has held the digits
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
+      for (int j = 0; j < RT; j++) {
+        const int r = 4 * j + t;
+        float l = l_run[j], z[G];
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float l = l_run[nt][e], z[G];
+        for (int h = 0; h < G; h++) z[h] = zacc[j][h];
 #pragma unroll
-          for (int h = 0; h < G; h++) z[h] = zacc[nt][h][e];
+        for (int o = 4; o < 32; o <<= 1) {
+          l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            l += __shfl_xor_sync(0xffffffffu, l, o);
-#pragma unroll
-            for (int h = 0; h < G; h++) z[h] += __shfl_xor_sync(0xffffffffu, z[h], o);
-          }
-          const int r = nt * 8 + 2 * t + e;
+          for (int h = 0; h < G; h++) z[h] += __shfl_xor_sync(0xffffffffu, z[h], o);
+        }
+        if (r < rows) {
           if (g == 0) {
-            ml[r] = m_run[nt][e];
+            ml[r] = m_run[j];
             ml[ROWS + r] = l;
           }
 #pragma unroll
           for (int h = 0; h < G; h++) {
             float* dst = merge + r * C::PITCH + 64 * h + 8 * g;
-            *reinterpret_cast<float4*>(dst) = make_float4(acc[nt][h][0][e] + z[h], acc[nt][h][1][e] + z[h], acc[nt][h][2][e] + z[h], acc[nt][h][3][e] + z[h]);
-            *reinterpret_cast<float4*>(dst + 4) =
-                make_float4(acc[nt][h][0][2 + e] + z[h], acc[nt][h][1][2 + e] + z[h], acc[nt][h][2][2 + e] + z[h], acc[nt][h][3][2 + e] + z[h]);
+            float o8[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              o8[i] = fmaf(acc[j / 2][h][i][RT == 1 ? h : j & 1], up, z[h]);
+              o8[4 + i] = fmaf(acc[j / 2][h][i][2 + (RT == 1 ? h : j & 1)], up, z[h]);
+            }
+            *reinterpret_cast<float4*>(dst) = make_float4(o8[0], o8[1], o8[2], o8[3]);
+            *reinterpret_cast<float4*>(dst + 4) = make_float4(o8[4], o8[5], o8[6], o8[7]);
           }
         }
       }
       group_sync();
-      const long long seg0 = qc - now.qi, seg1 = seg0 + now.s.quanta;  // the segment's quanta
-      const long long w0 = seg0 / per, w1 = (seg1 - 1) / per;          // the groups that share it
+      const int seg0 = now.piece - now.qi / PIECE, seg1 = seg0 + (now.s.quanta + PIECE - 1) / PIECE;  // the segment's pieces
+      const int w0 = seg0 / per, w1 = (seg1 - 1) / per;                                              // the groups that share it
       const bool whole = w0 == w1;
       const int slot = seg0 < q0 ? 0 : 1;
       float* part = p.part + ((int64_t)me * 2 + slot) * ROWS * (H + 2);
       const int tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
-      const int rows = min(ROWS, now.s.n * p.R - now.chunk * ROWS);
       auto store = [&](int r, int d, float inv, float a, float b) {
         const int row = now.chunk * ROWS + r;
         uint16_t* dst = p.out + ((int64_t)(tok0 + row / p.R) * p.Nq + now.n * p.R + row % p.R) * H + d;
-        *reinterpret_cast<uint32_t*>(dst) = i4_pack(a * inv, b * inv);
+        *reinterpret_cast<uint32_t*>(dst) = i4_pack_bf16(a * inv, b * inv);
       };
       for (int i = gtid; i < rows * (H / 2); i += GW * 32) {
         const int r = i / (H / 2), d = i % (H / 2) * 2;
@@ -542,15 +663,32 @@ __global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(
           for (int i = gtid; i < rows * (H / 2); i += GW * 32) {
             const int r = i / (H / 2), d = i % (H / 2) * 2;
             float m = -INFINITY, l = 0.0f, a = 0.0f, b = 0.0f;
-            for (long long k = w0; k <= w1; k++) {
-              const float* o = p.part + ((int64_t)k * 2 + (seg0 < k * per ? 0 : 1)) * ROWS * (H + 2) + r * (H + 2);
-              const float2 ml2 = __ldcg(reinterpret_cast<const float2*>(o)), v = __ldcg(reinterpret_cast<const float2*>(o + 2 + d));
-              if (ml2.x == -INFINITY) continue;
-              const float m_new = fmaxf(m, ml2.x), fo = i4_ex2(m - m_new), fn = i4_ex2(ml2.x - m_new);
-              l = l * fo + ml2.y * fn;
-              a = a * fo + v.x * fn;
-              b = b * fo + v.y * fn;
+            constexpr int U = 8;  // parts whose loads are in flight together
+            for (int k0 = w0; k0 <= w1; k0 += U) {
+              float2 ml2[U], v[U];
+#pragma unroll
+              for (int k = 0; k < U; k++) {
+                const int q = min(k0 + k, w1);
+                const float* o = p.part + ((int64_t)q * 2 + (seg0 < q * per ? 0 : 1)) * ROWS * (H + 2) + r * (H + 2);
+                ml2[k] = __ldcg(reinterpret_cast<const float2*>(o));
+                v[k] = __ldcg(reinterpret_cast<const float2*>(o + 2 + d));
+              }
+              float m_new = m;
+#pragma unroll
+              for (int k = 0; k < U; k++) m_new = fmaxf(m_new, ml2[k].x);
+              const float base = m_new == -INFINITY ? 0.0f : m_new, fo = i4_ex2(m - base);
+              l *= fo;
+              a *= fo;
+              b *= fo;
               m = m_new;
+#pragma unroll
+              for (int k = 0; k < U; k++) {
+                if (k0 + k > w1 || ml2[k].x == -INFINITY) continue;
+                const float f = i4_ex2(ml2[k].x - base);
+                l = fmaf(ml2[k].y, f, l);
+                a = fmaf(v[k].x, f, a);
+                b = fmaf(v[k].y, f, b);
+              }
             }
             store(r, d, m == -INFINITY ? 0.0f : 1.0f / l, a, b);
           }
@@ -559,27 +697,35 @@ __global__ void __launch_bounds__(I4Cfg<H, NT>::WARPS * 32, 1) int4_attn_kernel(
       group_sync();  // the buffers are free again
       fresh = true;
     }
-    if (qc + 1 < q1) advance(now);
+    advance(now);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- host side
-static int i4_tiles(int64_t T, int64_t B, int64_t Nq, int64_t Nkv) { return (T > B ? 2 : 1) * (Nq / Nkv) > 8 ? 2 : 1; }
-static size_t i4_scratch(int nt, int64_t H) { return (size_t)sm_count() * kI4Warps * (8 + 2 * (size_t)(8 * nt) * (H + 2) * 4); }
+// Query rows per lane: chunks of 4, 8 or 16 rows, the least that holds a sequence's rows where every sequence has one token (or two, where some have more)
+static int i4_rows(int64_t T, int64_t B, int64_t Nq, int64_t Nkv) {
+  const int64_t rows = (T > B ? 2 : 1) * (Nq / Nkv);
+  return rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
+}
+static size_t i4_scratch(int rt, int64_t H) { return (size_t)sm_count() * kI4Warps * (8 + 2 * (size_t)(4 * rt) * (H + 2) * 4); }
 
-template <int H, int NT>
+template <int H, int RT>
 static int i4_launch(I4Params& p, cudaStream_t st) {
-  using C = I4Cfg<H, NT>;
+  using C = I4Cfg<H, RT>;
   static bool opted[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !opted[dev]) {
-    TPX_CUDA_OK(cudaFuncSetAttribute(int4_attn_kernel<H, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    TPX_CUDA_OK(cudaFuncSetAttribute(int4_attn_kernel<H, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     if (dev >= 0 && dev < 16) opted[dev] = true;
   }
-  p.GW = C::WARPS;
-  TPX_CUDA_OK(launch_pdl(int4_attn_kernel<H, NT>, dim3(sm_count()), dim3(C::WARPS * 32), C::SMEM, st, p));
+  const int64_t most = ((int64_t)p.T * p.R / C::ROWS + p.c.B) * p.c.Nkv * (p.c.cols + C::WARPS);
+  TPX_REQUIRE(most < (1ll << 31), TPX_ERR_UNSUPPORTED, "int4_attention: more than 2^31 pages may be walked in one call");
+  // Segments enough for every group of four warps, or every warp, on its own: then groups are small, since short sequences fill few pages
+  const int64_t segments = (int64_t)p.c.B * p.c.Nkv;
+  p.GW = segments < 2 * sm_count() ? C::WARPS : segments < 16 * sm_count() ? 4 : 1;
+  TPX_CUDA_OK(launch_pdl(int4_attn_kernel<H, RT>, dim3(sm_count()), dim3(C::WARPS * 32), C::SMEM, st, p));
   return TPX_OK;
 }
 
@@ -589,7 +735,7 @@ using namespace tpx;
 
 extern "C" size_t tpx_int4_attention_scratch_bytes(int64_t T, int64_t B, int64_t Nq, int64_t kv_heads, int64_t H) {
   if (T <= 0 || kv_heads <= 0 || Nq <= 0) return 0;
-  return i4_scratch(i4_tiles(T, B, Nq, kv_heads), H);
+  return i4_scratch(i4_rows(T, B, Nq, kv_heads), H);
 }
 
 extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
@@ -603,9 +749,9 @@ extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
   TPX_REQUIRE(a->Nq > 0 && a->Nq <= 4096 && a->Nq % Nkv == 0, TPX_ERR_ARG, "int4_attention: %ld query heads for %ld key heads", (long)a->Nq, (long)Nkv);
   TPX_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->out) & 15) == 0 && a->ldq % 8 == 0, TPX_ERR_ARG, "int4_attention: q, its rows and out must be 16-byte aligned");
   if (a->T == 0) return TPX_OK;
-  const int nt = i4_tiles(a->T, a->cache->B, a->Nq, Nkv);
-  TPX_REQUIRE(a->scratch && ((uintptr_t)a->scratch & 255) == 0 && a->scratch_bytes >= i4_scratch(nt, H), TPX_ERR_SCRATCH,
-              "int4_attention: scratch of %zu bytes, %zu are needed (256-byte aligned)", a->scratch_bytes, i4_scratch(nt, H));
+  const int rt = i4_rows(a->T, a->cache->B, a->Nq, Nkv);
+  TPX_REQUIRE(a->scratch && ((uintptr_t)a->scratch & 255) == 0 && a->scratch_bytes >= i4_scratch(rt, H), TPX_ERR_SCRATCH,
+              "int4_attention: scratch of %zu bytes, %zu are needed (256-byte aligned)", a->scratch_bytes, i4_scratch(rt, H));
   // a number of its own for every call: 48 bits, from an origin that differs between processes
   static unsigned long long calls = 0;
   static const unsigned long long origin = (unsigned long long)(uintptr_t)&calls * 0x9E3779B97F4A7C15ull;
@@ -623,6 +769,6 @@ extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
   p.causal = a->causal;
   p.sc2 = a->scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
-  if (H == 128) return nt == 1 ? i4_launch<128, 1>(p, st) : i4_launch<128, 2>(p, st);
-  return nt == 1 ? i4_launch<64, 1>(p, st) : i4_launch<64, 2>(p, st);
+  if (H == 128) return rt == 1 ? i4_launch<128, 1>(p, st) : rt == 2 ? i4_launch<128, 2>(p, st) : i4_launch<128, 4>(p, st);
+  return rt == 1 ? i4_launch<64, 1>(p, st) : rt == 2 ? i4_launch<64, 2>(p, st) : i4_launch<64, 4>(p, st);
 }
