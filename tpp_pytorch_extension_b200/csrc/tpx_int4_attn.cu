@@ -187,8 +187,10 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
       totals[k] += scan[k][i];
     }
   }
-  const bool few = totals[0] <= kI4Piece * workers;
-  const int PIECE = few ? kI4Piece : 1;
+  const bool few = totals[1] <= workers;
+  const int shift = few ? 2 : 0;  // log2 of a piece's quanta
+  static_assert(kI4Piece == 4, "shift");
+  auto pieces_of = [&](int quanta) { return (quanta + (1 << shift) - 1) >> shift; };
   const int total = few ? totals[1] : totals[0], held_here = few ? mine[1] : mine[0], excl = few ? before[1] + incl[1] - mine[1] : before[0] + incl[0] - mine[0];
   const int per = (total + workers - 1) / workers;
   // where each group starts: the thread whose sequences hold that piece says so
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
       int acc = excl;
       for (int b = b_lo; b < b_hi; b++) {
         const I4Seq s = i4_seq(p, b, ROWS);
-        const int n = (int)((s.quanta + PIECE - 1) / PIECE) * s.chunks * p.c.Nkv;
+        const int n = pieces_of(s.quanta) * s.chunks * p.c.Nkv;
         if (s0 < acc + n) {
           start_b[k] = b;
           start_off[k] = s0 - acc;
@@ -212,41 +214,55 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   const int q0 = me * per, q1 = min(q0 + per, total);
   if (q0 >= q1) return;  // whole groups leave; what follows synchronises groups only
 
-  // ---- iterators over the quanta of the share
-  struct Iter {
-    int b, n, chunk, qi;  // sequence, key head, row chunk, quantum of the segment
-    int piece;      // of all pieces
-    I4Seq s;
+  // ---- the share as runs: parts of one segment each
+  struct Run {
+    int b, n, chunk, seg0;     // sequence (-1: none left), key head, row chunk, first piece of the segment among all pieces
+    int qi, qend, left;        // quanta of the segment, pieces of the share behind this run
+    int keys, quanta, chunks;  // of the sequence
   };
-  auto advance = [&](Iter& i) {
-    if (++i.qi < i.s.quanta) {
-      if (i.qi % PIECE == 0) i.piece++;
+  auto clip = [&](Run& r, int piece) {  // the run starts at that piece of the segment
+    const int take = min(pieces_of(r.quanta) - piece, r.left);
+    r.left -= take;
+    r.qi = piece << shift;
+    r.qend = min(r.quanta, (piece + take) << shift);
+  };
+  auto enter = [&](Run& r) {
+    const I4Seq s = i4_seq(p, r.b, ROWS);
+    r.keys = s.keys;
+    r.quanta = s.quanta;
+    r.chunks = s.chunks;
+  };
+  auto next = [&](Run& r) {
+    if (r.left == 0) {
+      r.b = -1;
       return;
     }
-    i.piece++;
-    i.qi = 0;
-    if (i.piece >= q1) return;
-    if (++i.chunk < i.s.chunks) return;
-    i.chunk = 0;
-    if (++i.n < p.c.Nkv) return;
-    i.n = 0;
-    do {
-      i.b++;
-      if (i.b >= p.c.B) return;
-      i.s = i4_seq(p, i.b, ROWS);
-    } while (i.s.quanta * i.s.chunks == 0);
+    r.seg0 += pieces_of(r.quanta);
+    if (++r.chunk == r.chunks) {
+      r.chunk = 0;
+      if (++r.n == p.c.Nkv) {
+        r.n = 0;
+        do {
+          if (++r.b >= p.c.B) {
+            r.b = -1;
+            return;
+          }
+          enter(r);
+        } while (r.quanta * r.chunks == 0);
+      }
+    }
+    clip(r, 0);
   };
-  Iter now;
+  Run now;
   {
     now.b = start_b[grp];
-    now.s = i4_seq(p, now.b, ROWS);
-    const int pieces = (now.s.quanta + PIECE - 1) / PIECE;
-    const int at = start_off[grp], per_head = (int)pieces * now.s.chunks;
-    now.n = (int)(at / per_head);
-    const int r = (int)(at % per_head);
-    now.chunk = r / pieces;
-    now.qi = r % pieces * PIECE;
-    now.piece = q0;
+    enter(now);
+    const int pieces = pieces_of(now.quanta), at = start_off[grp], segment = at / pieces, piece = at % pieces;
+    now.n = segment / now.chunks;
+    now.chunk = segment % now.chunks;
+    now.seg0 = q0 - piece;
+    now.left = q1 - q0;
+    clip(now, piece);
   }
 
   unsigned char* base = i4_smem + warp * C::WARP_BYTES;
@@ -254,36 +270,38 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   float* merge = reinterpret_cast<float*>(base + C::STAGES * L::BYTES);
   unsigned char* group_base = i4_smem + grp * GW * C::WARP_BYTES + C::STAGES * L::BYTES;
 
-  // The table's entry for this warp's page of an iterator's quantum, asked for one round before it is needed (-1: no page)
-  auto entry = [&](const Iter& i) -> int {
-    const int pg = i.qi * GW + w;
-    return i.piece < q1 && pg * kI4Page < i.s.keys ? p.c.table[(int64_t)i.b * p.c.cols + pg] : -1;
+  // The table's entry for this warp's page of a run's quantum, asked for one round before it is needed (-1: no page)
+  auto entry = [&](const Run& r) -> int {
+    const int pg = r.qi * GW + w;
+    return r.b >= 0 && pg * kI4Page < r.keys ? p.c.table[(int64_t)r.b * p.c.cols + pg] : -1;
   };
   // Fetches that page; the keys that it holds (0: no page)
-  auto fetch = [&](const Iter& i, int page, int stage) -> int {
-    if (page < 0 || page >= p.c.pages) return 0;
-    const uint8_t* src = p.c.pool + ((int64_t)page * p.c.Nkv + i.n) * L::BYTES + lane * 16;
+  auto fetch = [&](const Run& r, int page, int stage) -> int {
+    if ((unsigned)page >= (unsigned)p.c.pages) return 0;
+    const uint8_t* src = p.c.pool + ((int64_t)page * p.c.Nkv + r.n) * L::BYTES + lane * 16;
     const uint32_t dst = ring + stage * L::BYTES + lane * 16;
 #pragma unroll
     for (int k = 0; k < L::BYTES / 512; k++) i4_cp16(dst + k * 512, src + k * 512);
     if (L::BYTES % 512 && lane < L::BYTES % 512 / 16) i4_cp16(dst + L::BYTES / 512 * 512, src + L::BYTES / 512 * 512);
-    return min(i.s.keys - (i.qi * GW + w) * kI4Page, kI4Page);
+    return min(r.keys - (r.qi * GW + w) * kI4Page, kI4Page);
+  };
+  auto step = [&](Run& r) {
+    if (r.b >= 0 && ++r.qi == r.qend) next(r);
   };
 
-  Iter ahead = now;
-  int ahead_page = entry(ahead);
-  int held[C::STAGES];
-  static_assert(C::STAGES == 2, "the first two pages");
+  Run ahead = now;
+  int ahead_page = entry(ahead), held[2];
+  static_assert(C::STAGES == 2, "held");
   {
-    const Iter first = ahead;
+    const Run first = ahead;
     const int first_page = ahead_page;
-    advance(ahead);
+    step(ahead);
     ahead_page = entry(ahead);  // both entries are asked for before either is used
     held[0] = fetch(first, first_page, 0);
     asm volatile("cp.async.commit_group;" ::: "memory");
     held[1] = fetch(ahead, ahead_page, 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (ahead.piece < q1) advance(ahead);
+    step(ahead);
     ahead_page = entry(ahead);
   }
 
@@ -291,20 +309,19 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   float qsc[RT], qs[RT][G];                // per row: 2^-k scale log2(e), and sums of q times scale log2(e)
   float acc[VT][G][4][4], zacc[RT][G], m_run[RT], l_run[RT];
   int klim[RT], klim_min = 0, vexp = -126;  // values are kept in units of 2^vexp
-  bool fresh = true;
   const int kr = (g >> 1) + 4 * (g & 1);   // row g of a 16-row tile is key kr of its first 8, row g + 8 of its last 8
 
-  for (int stage = 0; now.piece < q1; stage = stage + 1 == C::STAGES ? 0 : stage + 1) {
-    if (fresh) {  // a new segment: its query rows, as digits, by the group together
-      fresh = false;
-      const int tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
+  int stage = 0;
+  for (; now.b >= 0; next(now)) {
+    const int n_tok = i4_seq(p, now.b, ROWS).n, tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
+    {  // the segment's query rows, as digits, by the group together
       constexpr int LR = H / 8;  // lanes per row
       uint2* frag = reinterpret_cast<uint2*>(group_base);
       float4* info = reinterpret_cast<float4*>(group_base + C::TILES * WPK * 256);
       for (int r0 = w * (32 / LR); r0 < ROWS; r0 += GW * (32 / LR)) {
         const int r = r0 + lane / LR, u = lane % LR, row = now.chunk * ROWS + r;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < ROWS && row < now.s.n * p.R)
+        if (r < ROWS && row < n_tok * p.R)
           v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(tok0 + row / p.R) * p.ldq + (int64_t)(now.n * p.R + row % p.R) * H + 8 * u);
         const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
         float x[8], top = 0.0f, sum = 0.0f, bad = 0.0f;
@@ -359,14 +376,14 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         qs[j][0] = f.y;
         if (G == 2) qs[j][G - 1] = f.z;
         // rows behind the last are computed with the last token's keys and not written
-        const int tok = min((now.chunk * ROWS + 4 * j + t) / p.R, now.s.n - 1);
-        klim[j] = p.causal ? (int)min(cap, first + tok + 1) : now.s.keys;
+        const int tok = min((now.chunk * ROWS + 4 * j + t) / p.R, n_tok - 1);
+        klim[j] = p.causal ? (int)min(cap, first + tok + 1) : now.keys;
         m_run[j] = -INFINITY;
         l_run[j] = 0.0f;
 #pragma unroll
         for (int h = 0; h < G; h++) zacc[j][h] = 0.0f;
       }
-      klim_min = p.causal ? (int)min(cap, first + now.chunk * ROWS / p.R + 1) : now.s.keys;
+      klim_min = p.causal ? (int)min(cap, first + now.chunk * ROWS / p.R + 1) : now.keys;
       vexp = -126;
 #pragma unroll
       for (int v = 0; v < VT; v++)
@@ -376,6 +393,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
           for (int i = 0; i < 4; i++) acc[v][h][i][0] = acc[v][h][i][1] = acc[v][h][i][2] = acc[v][h][i][3] = 0.0f;
     }
 
+    for (; now.qi < now.qend; now.qi++) {
     asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
     __syncwarp();
     const int have = held[0];
@@ -558,17 +576,16 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
       }
     }
     __syncwarp();  // the stage has been read by every lane
-#pragma unroll
-    for (int s = 0; s + 1 < C::STAGES; s++) held[s] = held[s + 1];
-    held[C::STAGES - 1] = fetch(ahead, ahead_page, stage);
+    held[0] = held[1];
+    held[1] = fetch(ahead, ahead_page, stage);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (ahead.piece < q1) advance(ahead);
+    step(ahead);
     ahead_page = entry(ahead);
+    stage ^= 1;
+    }
 
-    const bool last_of_segment = now.qi + 1 == now.s.quanta;
-    if (last_of_segment || (now.piece + 1 == q1 && (now.qi + 1) % PIECE == 0)) {
-      // ---- this group's part of the segment: rows of (maximum, sum, output), merged over its warps
-      const int rows = min(ROWS, now.s.n * p.R - now.chunk * ROWS);
+    {
+      const int rows = min(ROWS, n_tok * p.R - now.chunk * ROWS);
       float* ml = merge + ROWS * C::PITCH;
       const float up = i4_pow2(min(vexp, 126));
       if (GW > 1) group_sync();  // the first warp's buffer has held the digits
@@ -604,12 +621,11 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         }
       }
       group_sync();
-      const int seg0 = now.piece - now.qi / PIECE, seg1 = seg0 + (now.s.quanta + PIECE - 1) / PIECE;  // the segment's pieces
+      const int seg0 = now.seg0, seg1 = seg0 + pieces_of(now.quanta);                                       // the segment's pieces
       const int w0 = seg0 / per, w1 = (seg1 - 1) / per;                                              // the groups that share it
       const bool whole = w0 == w1;
       const int slot = seg0 < q0 ? 0 : 1;
       float* part = p.part + ((int64_t)me * 2 + slot) * ROWS * (H + 2);
-      const int tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
       auto store = [&](int r, int d, float inv, float a, float b) {
         const int row = now.chunk * ROWS + r;
         uint16_t* dst = p.out + ((int64_t)(tok0 + row / p.R) * p.Nq + now.n * p.R + row % p.R) * H + d;
@@ -695,17 +711,15 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         }
       }
       group_sync();  // the buffers are free again
-      fresh = true;
     }
-    advance(now);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- host side
-// Query rows per lane: chunks of 4, 8 or 16 rows, the least that holds a sequence's rows where every sequence has one token (or two, where some have more)
+// Query rows per lane: chunks of 4, 8 or 16 rows, the least that holds a sequence's rows if all have as many tokens
 static int i4_rows(int64_t T, int64_t B, int64_t Nq, int64_t Nkv) {
-  const int64_t rows = (T > B ? 2 : 1) * (Nq / Nkv);
+  const int64_t rows = (T + B - 1) / B * (Nq / Nkv);
   return rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
 }
 static size_t i4_scratch(int rt, int64_t H) { return (size_t)sm_count() * kI4Warps * (8 + 2 * (size_t)(4 * rt) * (H + 2) * 4); }
@@ -724,7 +738,7 @@ static int i4_launch(I4Params& p, cudaStream_t st) {
   TPX_REQUIRE(most < (1ll << 31), TPX_ERR_UNSUPPORTED, "int4_attention: more than 2^31 pages may be walked in one call");
   // Segments enough for every group of four warps, or every warp, on its own: then groups are small, since short sequences fill few pages
   const int64_t segments = (int64_t)p.c.B * p.c.Nkv;
-  p.GW = segments < 2 * sm_count() ? C::WARPS : segments < 16 * sm_count() ? 4 : 1;
+  p.GW = segments < sm_count() ? C::WARPS : segments < 8 * sm_count() ? 4 : 1;
   TPX_CUDA_OK(launch_pdl(int4_attn_kernel<H, RT>, dim3(sm_count()), dim3(C::WARPS * 32), C::SMEM, st, p));
   return TPX_OK;
 }
@@ -734,7 +748,7 @@ static int i4_launch(I4Params& p, cudaStream_t st) {
 using namespace tpx;
 
 extern "C" size_t tpx_int4_attention_scratch_bytes(int64_t T, int64_t B, int64_t Nq, int64_t kv_heads, int64_t H) {
-  if (T <= 0 || kv_heads <= 0 || Nq <= 0) return 0;
+  if (T <= 0 || B <= 0 || kv_heads <= 0 || Nq <= 0) return 0;
   return i4_scratch(i4_rows(T, B, Nq, kv_heads), H);
 }
 
