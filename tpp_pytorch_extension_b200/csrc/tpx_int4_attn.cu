@@ -34,7 +34,7 @@ struct I4Params {
   unsigned long long* counters;  // [workers]
   unsigned long long nonce;      // low 16 bits zero
   int64_t ldq;
-  int T, Nq, R, GW, causal;
+  int T, Nq, R, causal;
   float sc2;                     // scale * log2(e)
 };
 
@@ -102,10 +102,10 @@ __device__ __forceinline__ void i4_lds(const unsigned char* a, uint32_t (&v)[N])
 }
 
 // Work of one sequence. A quantum is GW pages, one per warp of a group; a piece is what is never cut between groups: one quantum, or
-// four where there is too little work for all groups anyway (two more quanta in a row cost less than adding up partial results).
-constexpr int kI4Piece = 4;
+// four where there is too little work for all groups anyway (more quanta in a row cost less than adding up partial results).
+constexpr int kI4PieceShift = 2;
 struct I4Seq {
-  int n, keys, quanta, chunks;  // tokens of the call, keys, quanta of a segment, row chunks
+  int n, keys, pages, chunks;  // tokens of the call, keys, their pages, row chunks
 };
 __device__ __forceinline__ I4Seq i4_seq(const I4Params& p, int b, int rows) {
   I4Seq s;
@@ -117,9 +117,21 @@ __device__ __forceinline__ I4Seq i4_seq(const I4Params& p, int b, int rows) {
   }
   const long long keys = (long long)max(p.c.lengths[b], 0) + s.n, cap = (long long)p.c.cols * kI4Page;
   s.keys = (int)min(keys, cap);
-  s.quanta = ((s.keys + kI4Page - 1) / kI4Page + p.GW - 1) / p.GW;
+  s.pages = (s.keys + kI4Page - 1) / kI4Page;
   s.chunks = (int)(((long long)s.n * p.R + rows - 1) / rows);
   return s;
+}
+// Counts one arrival at a segment of `want` parts; whether it is the last. The word starts as anything but this call's number (that of another
+// call, or none): who finds that (`was`: what it held some time ago) sets it up by one exchange, which fails only where another has; then
+// everyone adds one. No retries: nineteen groups that finish together took 14 us to count themselves by compare-and-swap. The
+// addition releases what the group has written before it met at a barrier, and acquires the others'.
+__device__ __forceinline__ bool i4_arrive(unsigned long long* word, unsigned long long was, unsigned long long nonce, unsigned want) {
+  if ((was & ~0xffffull) != nonce) atomicCAS(word, was, nonce);
+  unsigned long long seen;
+  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], %2;" : "=l"(seen) : "l"(word), "l"(1ull) : "memory");
+  const bool last = (unsigned)(seen & 0xffffull) + 1 == want;
+  if (last) *reinterpret_cast<volatile unsigned long long*>(word) = 0;  // a replayed call starts anew
+  return last;
 }
 
 // RT: query rows per lane, 4 RT in a chunk
@@ -127,7 +139,8 @@ template <int H, int RT>
 struct I4Cfg {
   static constexpr int ROWS = 4 * RT;
   static constexpr int STAGES = 2;
-  static constexpr int WARPS = RT < 4 ? kI4Warps : kI4Warps / 2;
+  static constexpr int WARP_SHIFT = RT < 4 ? 4 : 3, WARPS = 1 << WARP_SHIFT;
+  static_assert(WARPS <= kI4Warps, "scratch");
   static constexpr int TILES = RT + (RT + 1) / 2;          // n-tiles of q digits: upper two of 4 rows each, lowest of 8
   static constexpr int PITCH = H + 4;                      // floats of a row in the merge buffer
   static constexpr int MERGE = (ROWS * PITCH + 2 * ROWS) * 4;
@@ -142,28 +155,58 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   using L = I4<H>;
   constexpr int ROWS = C::ROWS, G = L::G, WPK = H / 32, VT = (RT + 1) / 2;  // WPK: words of a lane per key row; VT: n-tiles of weights
   extern __shared__ __align__(16) unsigned char i4_smem[];
-  __shared__ int scan[2][C::WARPS], start_off[C::WARPS];
+  __shared__ int scan[3][C::WARPS], start_off[C::WARPS];
   __shared__ int start_b[C::WARPS];
   pdl_trigger();
   pdl_wait();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int GW = p.GW, grp = warp / GW, w = warp % GW, gtid = threadIdx.x - grp * GW * 32;
-  const int workers = (int)gridDim.x * (C::WARPS / GW), me = (int)blockIdx.x * (C::WARPS / GW) + grp;
+
+  // ---- how many segments, how many pages, how many at most in one
+  const int per_thread = (p.c.B + blockDim.x - 1) / blockDim.x;
+  const int b_lo = min((int)threadIdx.x * per_thread, p.c.B), b_hi = min(b_lo + per_thread, p.c.B);
+  int segments = 0, all_pages = 0, most_pages = 0;
+  for (int b = b_lo; b < b_hi; b++) {
+    const I4Seq s = i4_seq(p, b, ROWS);
+    segments += s.chunks * p.c.Nkv;
+    all_pages += s.chunks * p.c.Nkv * s.pages;
+    if (s.chunks) most_pages = max(most_pages, s.pages);
+  }
+  segments = __reduce_add_sync(0xffffffffu, segments);
+  all_pages = __reduce_add_sync(0xffffffffu, all_pages);
+  most_pages = __reduce_max_sync(0xffffffffu, most_pages);
+  if (lane == 0) {
+    scan[0][warp] = segments;
+    scan[1][warp] = all_pages;
+    scan[2][warp] = most_pages;
+  }
+  __syncthreads();
+  segments = all_pages = most_pages = 0;
+  for (int i = 0; i < C::WARPS; i++) {
+    segments += scan[0][i];
+    all_pages += scan[1][i];
+    most_pages = max(most_pages, scan[2][i]);
+  }
+  // Warps work on segments of their own where there are segments enough and none is so long that adding up its parts would take
+  // long: no warp waits for another. Else groups of four, or the whole block: its warps' results meet in shared memory
+  const int even = (all_pages + (int)gridDim.x * C::WARPS - 1) / ((int)gridDim.x * C::WARPS);  // pages per warp
+  const bool many = segments >= (int)gridDim.x;
+  const int gsh = !many ? C::WARP_SHIFT : most_pages <= 8 * even ? 0 : most_pages <= 64 * even ? 2 : C::WARP_SHIFT, GW = 1 << gsh;
+  const int grp = warp >> gsh, w = warp & (GW - 1), gtid = threadIdx.x - grp * GW * 32;
+  const int workers = (int)gridDim.x * (C::WARPS >> gsh), me = (int)blockIdx.x * (C::WARPS >> gsh) + grp;
   auto group_sync = [&]() {
     if (GW == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(GW * 32) : "memory");
   };
 
   // ---- the pieces of all segments, and this group's share of them
-  const int per_thread = (p.c.B + blockDim.x - 1) / blockDim.x;
-  const int b_lo = min((int)threadIdx.x * per_thread, p.c.B), b_hi = min(b_lo + per_thread, p.c.B);
+  auto quanta_of = [&](int pages) { return (pages + GW - 1) >> gsh; };
   int mine[2] = {0, 0};  // in pieces of one quantum, of four
   for (int b = b_lo; b < b_hi; b++) {
     const I4Seq s = i4_seq(p, b, ROWS);
-    const int segments = (int)s.chunks * p.c.Nkv;
-    mine[0] += segments * s.quanta;
-    mine[1] += segments * ((s.quanta + kI4Piece - 1) / kI4Piece);
+    const int n = s.chunks * p.c.Nkv, quanta = quanta_of(s.pages);
+    mine[0] += n * quanta;
+    mine[1] += n * ((quanta + (1 << kI4PieceShift) - 1) >> kI4PieceShift);
   }
   int incl[2] = {mine[0], mine[1]};
 #pragma unroll
@@ -174,6 +217,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
       if (lane >= o) incl[k] += v;
     }
   }
+  __syncthreads();
   if (lane == 31) {
     scan[0][warp] = incl[0];
     scan[1][warp] = incl[1];
@@ -188,19 +232,18 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     }
   }
   const bool few = totals[1] <= workers;
-  const int shift = few ? 2 : 0;  // log2 of a piece's quanta
-  static_assert(kI4Piece == 4, "shift");
+  const int shift = few ? kI4PieceShift : 0;  // log2 of a piece's quanta
   auto pieces_of = [&](int quanta) { return (quanta + (1 << shift) - 1) >> shift; };
   const int total = few ? totals[1] : totals[0], held_here = few ? mine[1] : mine[0], excl = few ? before[1] + incl[1] - mine[1] : before[0] + incl[0] - mine[0];
   const int per = (total + workers - 1) / workers;
   // where each group starts: the thread whose sequences hold that piece says so
-  for (int k = 0; k < C::WARPS / GW; k++) {
-    const int s0 = ((int)blockIdx.x * (C::WARPS / GW) + k) * per;
+  for (int k = 0; k < C::WARPS >> gsh; k++) {
+    const int s0 = ((int)blockIdx.x * (C::WARPS >> gsh) + k) * per;
     if (s0 < total && excl <= s0 && s0 < excl + held_here) {
       int acc = excl;
       for (int b = b_lo; b < b_hi; b++) {
         const I4Seq s = i4_seq(p, b, ROWS);
-        const int n = pieces_of(s.quanta) * s.chunks * p.c.Nkv;
+        const int n = pieces_of(quanta_of(s.pages)) * s.chunks * p.c.Nkv;
         if (s0 < acc + n) {
           start_b[k] = b;
           start_off[k] = s0 - acc;
@@ -229,7 +272,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   auto enter = [&](Run& r) {
     const I4Seq s = i4_seq(p, r.b, ROWS);
     r.keys = s.keys;
-    r.quanta = s.quanta;
+    r.quanta = quanta_of(s.pages);
     r.chunks = s.chunks;
   };
   auto next = [&](Run& r) {
@@ -314,6 +357,10 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   int stage = 0;
   for (; now.b >= 0; next(now)) {
     const int n_tok = i4_seq(p, now.b, ROWS).n, tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
+    const int w0 = now.seg0 / per, w1 = (now.seg0 + pieces_of(now.quanta) - 1) / per;  // the groups that share the segment
+    const bool whole = w0 == w1;
+    unsigned long long word_was = 0;
+    if (!whole && gtid == 0) word_was = *reinterpret_cast<volatile unsigned long long*>(p.counters + w0);
     {  // the segment's query rows, as digits, by the group together
       constexpr int LR = H / 8;  // lanes per row
       uint2* frag = reinterpret_cast<uint2*>(group_base);
@@ -324,7 +371,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         if (r < ROWS && row < n_tok * p.R)
           v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(tok0 + row / p.R) * p.ldq + (int64_t)(now.n * p.R + row % p.R) * H + 8 * u);
         const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-        float x[8], top = 0.0f, sum = 0.0f, bad = 0.0f;
+        float x[8], top = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           x[2 * i] = __uint_as_float(vw[i] << 16);
@@ -332,29 +379,34 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          top = fmaxf(top, fabsf(x[i]));
+          asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x[i])));
           sum += x[i];
-          bad = fmaf(x[i], 0.0f, bad);  // a NaN where any value is not finite
         }
 #pragma unroll
         for (int o = LR / 2; o > 0; o >>= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          bad += __shfl_xor_sync(0xffffffffu, bad, o);
+          const float v2 = __shfl_xor_sync(0xffffffffu, top, o);
+          asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(v2));
           if (o < 8) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // within a group of 64
         }
         const float other = __shfl_xor_sync(0xffffffffu, sum, LR / 2);
-        // top * 2^k in [2^19, 2^20): 20 bits
+        // top * 2^k in [2^19, 2^20): Q = hi 2^14 + mid 2^7 + lo, -64 <= hi < 64, 0 <= mid, lo < 128, read off the bits of 1.5 * 2^23 + Q
         const int k = min(19 - ((int)((__float_as_uint(top) >> 23) & 255) - 127), 120);
         const float up = i4_pow2(k);
-        uint32_t d[3][2] = {};  // digits: bytes of the even and of the odd values
+        uint32_t d[3][2];  // digits: bytes of the even and of the odd values
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int Q = (int)(__float_as_uint(fmaf(x[i], up, __uint_as_float(kI4Magic))) - kI4Magic);
-          const int hi = (Q + 8192) >> 14, rem = Q - (hi << 14), mid = (rem + 64) >> 7, lo = rem - (mid << 7);
-          d[0][i & 1] |= (uint32_t)(hi & 255) << (8 * (i >> 1));
-          d[1][i & 1] |= (uint32_t)(mid & 255) << (8 * (i >> 1));
-          d[2][i & 1] |= (uint32_t)(lo & 255) << (8 * (i >> 1));
+        for (int odd = 0; odd < 2; odd++) {
+          uint32_t b[4];   // digits of a value in its bytes 0..2
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t Q = __float_as_uint(fmaf(x[2 * i + odd], up, __uint_as_float(kI4Magic)));
+            b[i] = (Q & 0x7fu) | ((Q << 1) & 0x7f00u) | ((Q << 2) & 0xff0000u);
+          }
+          const uint32_t p01 = __byte_perm(b[0], b[1], 0x5140), p23 = __byte_perm(b[2], b[3], 0x5140);
+          d[2][odd] = __byte_perm(p01, p23, 0x5410);
+          d[1][odd] = __byte_perm(p01, p23, 0x7632);
+          d[0][odd] = __byte_perm(__byte_perm(b[0], b[1], 0x0062), __byte_perm(b[2], b[3], 0x0062), 0x5410);
         }
+        const float bad = top * 0.0f;  // a NaN where any value is not finite
         if (r < ROWS) {
           const int tile = r / 4, col = 2 * (r % 4), i = u / 4, tt = u % 4;
           frag[(tile * WPK + i) * 32 + col * 4 + tt] = make_uint2(d[0][0], d[0][1]);
@@ -584,134 +636,223 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     stage ^= 1;
     }
 
+    // ---- the run's end: rows of (maximum, sum, output); a lane has 8 dimensions 64 h + 8 g + .. of the rows 4 j + t
+    const int rows = min(ROWS, n_tok * p.R - now.chunk * ROWS);
+    // A part is [RT][G][2][32 lanes] float4 as the lanes have them, then maxima and sums; one of a share's first, one of its last segment
+    auto part_of = [&](int k) { return p.part + ((int64_t)k * 2 + (now.seg0 < k * per ? 0 : 1)) * ROWS * (H + 2); };
+    auto row_out = [&](int r) {
+      const int row = now.chunk * ROWS + r;
+      return p.out + ((int64_t)(tok0 + row / p.R) * p.Nq + now.n * p.R + row % p.R) * H;
+    };
+    float o[RT][G][8];
     {
-      const int rows = min(ROWS, n_tok * p.R - now.chunk * ROWS);
-      float* ml = merge + ROWS * C::PITCH;
       const float up = i4_pow2(min(vexp, 126));
-      if (GW > 1) group_sync();  // the first warp's buffer has held the digits
+#pragma unroll
+      for (int j = 0; j < RT; j++) {
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) {
+          l_run[j] += __shfl_xor_sync(0xffffffffu, l_run[j], k);
+#pragma unroll
+          for (int h = 0; h < G; h++) zacc[j][h] += __shfl_xor_sync(0xffffffffu, zacc[j][h], k);
+        }
+#pragma unroll
+        for (int h = 0; h < G; h++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            o[j][h][i] = fmaf(acc[j / 2][h][i][RT == 1 ? h : j & 1], up, zacc[j][h]);
+            o[j][h][4 + i] = fmaf(acc[j / 2][h][i][2 + (RT == 1 ? h : j & 1)], up, zacc[j][h]);
+          }
+      }
+    }
+    auto write_out = [&]() {
+#pragma unroll
+      for (int j = 0; j < RT; j++) {
+        if (4 * j + t >= rows) continue;
+        const float inv = m_run[j] == -INFINITY ? 0.0f : 1.0f / l_run[j];
+        uint16_t* dst = row_out(4 * j + t);
+#pragma unroll
+        for (int h = 0; h < G; h++) {
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = i4_pack_bf16(o[j][h][2 * i] * inv, o[j][h][2 * i + 1] * inv);
+          *reinterpret_cast<uint4*>(dst + 64 * h + 8 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+    };
+    if (GW == 1) {
+      if (whole) {
+        write_out();
+      } else {
+        float* part = part_of(me);
+#pragma unroll
+        for (int j = 0; j < RT; j++) {
+#pragma unroll
+          for (int h = 0; h < G; h++)
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+              reinterpret_cast<float4*>(part)[((j * G + h) * 2 + q) * 32 + lane] = make_float4(o[j][h][4 * q], o[j][h][4 * q + 1], o[j][h][4 * q + 2], o[j][h][4 * q + 3]);
+          if (g == 0) {
+            part[ROWS * H + 4 * j + t] = m_run[j];
+            part[ROWS * H + ROWS + 4 * j + t] = l_run[j];
+          }
+        }
+        __syncwarp();
+        bool last = false;
+        if (lane == 0) last = i4_arrive(p.counters + w0, word_was, p.nonce, (unsigned)(w1 - w0 + 1));
+        if (__shfl_sync(0xffffffffu, (int)last, 0)) {
+#pragma unroll
+          for (int j = 0; j < RT; j++) {
+            m_run[j] = -INFINITY;
+            l_run[j] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < G; h++)
+#pragma unroll
+              for (int i = 0; i < 8; i++) o[j][h][i] = 0.0f;
+          }
+#pragma unroll 2
+          for (int k = w0; k <= w1; k++) {
+            const float* from = part_of(k);
+            float4 v[RT][G][2];
+            float pm[RT], pl[RT];
+#pragma unroll
+            for (int j = 0; j < RT; j++) {
+              pm[j] = __ldcg(from + ROWS * H + 4 * j + t);
+              pl[j] = __ldcg(from + ROWS * H + ROWS + 4 * j + t);
+#pragma unroll
+              for (int h = 0; h < G; h++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) v[j][h][q] = __ldcg(reinterpret_cast<const float4*>(from) + ((j * G + h) * 2 + q) * 32 + lane);
+            }
+#pragma unroll
+            for (int j = 0; j < RT; j++) {
+              if (pm[j] == -INFINITY) continue;  // saw nothing of this row
+              const float m_new = fmaxf(m_run[j], pm[j]), fo = i4_ex2(m_run[j] - m_new), fn = i4_ex2(pm[j] - m_new);
+              m_run[j] = m_new;
+              l_run[j] = fmaf(l_run[j], fo, pl[j] * fn);
+#pragma unroll
+              for (int h = 0; h < G; h++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                  const float x4[4] = {v[j][h][q].x, v[j][h][q].y, v[j][h][q].z, v[j][h][q].w};
+#pragma unroll
+                  for (int i = 0; i < 4; i++) o[j][h][4 * q + i] = fmaf(o[j][h][4 * q + i], fo, x4[i] * fn);
+                }
+            }
+          }
+          write_out();
+        }
+      }
+    } else {
+      float* ml = merge + ROWS * C::PITCH;
+      group_sync();  // the first warp's buffer has held the digits
 #pragma unroll
       for (int j = 0; j < RT; j++) {
         const int r = 4 * j + t;
-        float l = l_run[j], z[G];
-#pragma unroll
-        for (int h = 0; h < G; h++) z[h] = zacc[j][h];
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          l += __shfl_xor_sync(0xffffffffu, l, o);
-#pragma unroll
-          for (int h = 0; h < G; h++) z[h] += __shfl_xor_sync(0xffffffffu, z[h], o);
-        }
         if (r < rows) {
           if (g == 0) {
             ml[r] = m_run[j];
-            ml[ROWS + r] = l;
+            ml[ROWS + r] = l_run[j];
           }
 #pragma unroll
-          for (int h = 0; h < G; h++) {
-            float* dst = merge + r * C::PITCH + 64 * h + 8 * g;
-            float o8[8];
+          for (int h = 0; h < G; h++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              o8[i] = fmaf(acc[j / 2][h][i][RT == 1 ? h : j & 1], up, z[h]);
-              o8[4 + i] = fmaf(acc[j / 2][h][i][2 + (RT == 1 ? h : j & 1)], up, z[h]);
-            }
-            *reinterpret_cast<float4*>(dst) = make_float4(o8[0], o8[1], o8[2], o8[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(o8[4], o8[5], o8[6], o8[7]);
-          }
+            for (int q = 0; q < 2; q++)
+              *reinterpret_cast<float4*>(merge + r * C::PITCH + 64 * h + 8 * g + 4 * q) =
+                  make_float4(o[j][h][4 * q], o[j][h][4 * q + 1], o[j][h][4 * q + 2], o[j][h][4 * q + 3]);
         }
       }
       group_sync();
-      const int seg0 = now.seg0, seg1 = seg0 + pieces_of(now.quanta);                                       // the segment's pieces
-      const int w0 = seg0 / per, w1 = (seg1 - 1) / per;                                              // the groups that share it
-      const bool whole = w0 == w1;
-      const int slot = seg0 < q0 ? 0 : 1;
-      float* part = p.part + ((int64_t)me * 2 + slot) * ROWS * (H + 2);
-      auto store = [&](int r, int d, float inv, float a, float b) {
-        const int row = now.chunk * ROWS + r;
-        uint16_t* dst = p.out + ((int64_t)(tok0 + row / p.R) * p.Nq + now.n * p.R + row % p.R) * H + d;
-        *reinterpret_cast<uint32_t*>(dst) = i4_pack_bf16(a * inv, b * inv);
+      float* part = part_of(me);
+      auto store = [&](int r, int d, float m, float l, const float4& v) {
+        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+        *reinterpret_cast<uint2*>(row_out(r) + d) = make_uint2(i4_pack_bf16(v.x * inv, v.y * inv), i4_pack_bf16(v.z * inv, v.w * inv));
       };
-      for (int i = gtid; i < rows * (H / 2); i += GW * 32) {
-        const int r = i / (H / 2), d = i % (H / 2) * 2;
-        float m = -INFINITY;
-        for (int k = 0; k < GW; k++) m = fmaxf(m, reinterpret_cast<float*>(group_base + k * C::WARP_BYTES)[ROWS * C::PITCH + r]);
+      auto add = [&](float4& v, float fo, const float4& x, float fn) {
+        v.x = fmaf(v.x, fo, x.x * fn);
+        v.y = fmaf(v.y, fo, x.y * fn);
+        v.z = fmaf(v.z, fo, x.z * fn);
+        v.w = fmaf(v.w, fo, x.w * fn);
+      };
+      for (int e = gtid; e < ROWS * H / 4; e += GW * 32) {  // in the order of a part
+        const int le = e & 31, q = (e >> 5) & 1, h = (e >> 6) % G, r = 4 * ((e >> 6) / G) + (le & 3), d = 64 * h + 8 * (le >> 2) + 4 * q;
+        if (r >= rows) continue;
+        float m = -INFINITY, l = 0.0f;
+        for (int k = 0; k < GW; k++) m = fmaxf(m, reinterpret_cast<const float*>(group_base + k * C::WARP_BYTES)[ROWS * C::PITCH + r]);
         const float ref = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, a = 0.0f, b = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < GW; k++) {
-          const float* o = reinterpret_cast<const float*>(group_base + k * C::WARP_BYTES);
-          const float f = i4_ex2(o[ROWS * C::PITCH + r] - ref);
-          if (o[ROWS * C::PITCH + r] == -INFINITY) continue;  // a warp that saw nothing of this row
-          l = fmaf(o[ROWS * C::PITCH + ROWS + r], f, l);
-          a = fmaf(o[r * C::PITCH + d], f, a);
-          b = fmaf(o[r * C::PITCH + d + 1], f, b);
+          const float* from = reinterpret_cast<const float*>(group_base + k * C::WARP_BYTES);
+          const float pm = from[ROWS * C::PITCH + r];
+          if (pm == -INFINITY) continue;  // a warp that saw nothing of this row
+          const float f = i4_ex2(pm - ref);
+          l = fmaf(from[ROWS * C::PITCH + ROWS + r], f, l);
+          add(v, 1.0f, *reinterpret_cast<const float4*>(from + r * C::PITCH + d), f);
         }
         if (whole) {
-          store(r, d, m == -INFINITY ? 0.0f : 1.0f / l, a, b);
+          store(r, d, m, l, v);
         } else {
+          reinterpret_cast<float4*>(part)[e] = v;
           if (d == 0) {
-            part[r * (H + 2)] = m;
-            part[r * (H + 2) + 1] = l;
+            part[ROWS * H + r] = m;
+            part[ROWS * H + ROWS + r] = l;
           }
-          *reinterpret_cast<float2*>(part + r * (H + 2) + 2 + d) = make_float2(a, b);
         }
       }
       if (!whole) {
-        __threadfence();
         group_sync();
-        int* flag = reinterpret_cast<int*>(group_base + ROWS * C::PITCH * 4 + 2 * ROWS * 4 - 4);  // the last float of the first warp's buffer: read by now
-        if (gtid == 0) {
-          unsigned long long* word = p.counters + w0;
-          const unsigned long long want = (unsigned long long)(w1 - w0 + 1);
-          unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(word), next;
-          for (;;) {  // lock-free: a failed exchange means that another group has arrived
-            next = (old & ~0xffffull) == p.nonce ? old + 1 : p.nonce + 1;
-            const unsigned long long seen = atomicCAS(word, old, next);
-            if (seen == old) break;
-            old = seen;
-          }
-          const bool last = (next & 0xffffull) == want;
-          if (last) *word = 0;  // a replayed call starts anew
-          *flag = last;
-          __threadfence();
-        }
+        int* flag = reinterpret_cast<int*>(group_base + (ROWS * C::PITCH + 2 * ROWS - 1) * 4);  // the last float of the first warp's buffer: read by now
+        if (gtid == 0) *flag = i4_arrive(p.counters + w0, word_was, p.nonce, (unsigned)(w1 - w0 + 1));
         group_sync();
         if (*flag) {
-          for (int i = gtid; i < rows * (H / 2); i += GW * 32) {
-            const int r = i / (H / 2), d = i % (H / 2) * 2;
-            float m = -INFINITY, l = 0.0f, a = 0.0f, b = 0.0f;
+          // the parts, by every thread of the group: a piece of four values each, or where there are more threads some of the parts each
+          constexpr int ITEMS = ROWS * H / 4;
+          const int splits = max(GW * 32 / ITEMS, 1), first = gtid / ITEMS;
+          for (int e = gtid % ITEMS; e < ITEMS; e += GW * 32) {
+            const int le = e & 31, q = (e >> 5) & 1, h = (e >> 6) % G, r = 4 * ((e >> 6) / G) + (le & 3), d = 64 * h + 8 * (le >> 2) + 4 * q;
+            float m = -INFINITY, l = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             constexpr int U = 8;  // parts whose loads are in flight together
-            for (int k0 = w0; k0 <= w1; k0 += U) {
-              float2 ml2[U], v[U];
+            for (int k0 = w0 + first; k0 <= w1; k0 += U * splits) {
+              float pm[U], pl[U];
+              float4 x[U];
 #pragma unroll
               for (int k = 0; k < U; k++) {
-                const int q = min(k0 + k, w1);
-                const float* o = p.part + ((int64_t)q * 2 + (seg0 < q * per ? 0 : 1)) * ROWS * (H + 2) + r * (H + 2);
-                ml2[k] = __ldcg(reinterpret_cast<const float2*>(o));
-                v[k] = __ldcg(reinterpret_cast<const float2*>(o + 2 + d));
+                const float* from = part_of(min(k0 + k * splits, w1));
+                pm[k] = __ldcg(from + ROWS * H + r);
+                pl[k] = __ldcg(from + ROWS * H + ROWS + r);
+                x[k] = __ldcg(reinterpret_cast<const float4*>(from) + e);
               }
-              float m_new = m;
-#pragma unroll
-              for (int k = 0; k < U; k++) m_new = fmaxf(m_new, ml2[k].x);
-              const float base = m_new == -INFINITY ? 0.0f : m_new, fo = i4_ex2(m - base);
-              l *= fo;
-              a *= fo;
-              b *= fo;
-              m = m_new;
 #pragma unroll
               for (int k = 0; k < U; k++) {
-                if (k0 + k > w1 || ml2[k].x == -INFINITY) continue;
-                const float f = i4_ex2(ml2[k].x - base);
-                l = fmaf(ml2[k].y, f, l);
-                a = fmaf(v[k].x, f, a);
-                b = fmaf(v[k].y, f, b);
+                if (k0 + k * splits > w1 || pm[k] == -INFINITY) continue;
+                const float m_new = fmaxf(m, pm[k]), fo = i4_ex2(m - m_new), fn = i4_ex2(pm[k] - m_new);
+                m = m_new;
+                l = fmaf(l, fo, pl[k] * fn);
+                add(v, fo, x[k], fn);
               }
             }
-            store(r, d, m == -INFINITY ? 0.0f : 1.0f / l, a, b);
+            if (splits > 1) {  // once around this loop: every thread has one item
+              float* mine_of = merge + lane * 6;
+              if (first > 0) {
+                mine_of[0] = m; mine_of[1] = l; mine_of[2] = v.x; mine_of[3] = v.y; mine_of[4] = v.z; mine_of[5] = v.w;
+              }
+              group_sync();
+              if (first > 0) break;
+              for (int k = 1; k < splits; k++) {
+                const float* from = reinterpret_cast<const float*>(group_base + (w + k * (ITEMS / 32)) * C::WARP_BYTES) + lane * 6;
+                if (from[0] == -INFINITY) continue;
+                const float m_new = fmaxf(m, from[0]), fo = i4_ex2(m - m_new), fn = i4_ex2(from[0] - m_new);
+                m = m_new;
+                l = fmaf(l, fo, from[1] * fn);
+                add(v, fo, make_float4(from[2], from[3], from[4], from[5]), fn);
+              }
+            }
+            if (r < rows) store(r, d, m, l, v);
           }
         }
       }
-      group_sync();  // the buffers are free again
     }
+    group_sync();  // the buffers are free again
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -736,9 +877,6 @@ static int i4_launch(I4Params& p, cudaStream_t st) {
   }
   const int64_t most = ((int64_t)p.T * p.R / C::ROWS + p.c.B) * p.c.Nkv * (p.c.cols + C::WARPS);
   TPX_REQUIRE(most < (1ll << 31), TPX_ERR_UNSUPPORTED, "int4_attention: more than 2^31 pages may be walked in one call");
-  // Segments enough for every group of four warps, or every warp, on its own: then groups are small, since short sequences fill few pages
-  const int64_t segments = (int64_t)p.c.B * p.c.Nkv;
-  p.GW = segments < sm_count() ? C::WARPS : segments < 8 * sm_count() ? 4 : 1;
   TPX_CUDA_OK(launch_pdl(int4_attn_kernel<H, RT>, dim3(sm_count()), dim3(C::WARPS * 32), C::SMEM, st, p));
   return TPX_OK;
 }
