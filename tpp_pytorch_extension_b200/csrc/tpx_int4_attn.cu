@@ -104,6 +104,9 @@ __device__ __forceinline__ void i4_lds(const unsigned char* a, uint32_t (&v)[N])
 // Work of one sequence. A quantum is GW pages, one per warp of a group; a piece is what is never cut between groups: one quantum, or
 // four where there is too little work for all groups anyway (more quanta in a row cost less than adding up partial results).
 constexpr int kI4PieceShift = 2;
+// Quanta that the start and the end of a run take the time of: without them a group that drew six short segments took 54 us where one
+// with a part of a long segment took 27 (64 sequences of 1 to 4096 tokens)
+constexpr int kI4Start = 2;
 struct I4Seq {
   int n, keys, pages, chunks;  // tokens of the call, keys, their pages, row chunks
 };
@@ -199,13 +202,13 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(GW * 32) : "memory");
   };
 
-  // ---- the pieces of all segments, and this group's share of them
+  // ---- the units of all segments, and this group's share of them
   auto quanta_of = [&](int pages) { return (pages + GW - 1) >> gsh; };
-  int mine[2] = {0, 0};  // in pieces of one quantum, of four
+  int mine[2] = {0, 0};  // in quanta, in pieces of four
   for (int b = b_lo; b < b_hi; b++) {
     const I4Seq s = i4_seq(p, b, ROWS);
     const int n = s.chunks * p.c.Nkv, quanta = quanta_of(s.pages);
-    mine[0] += n * quanta;
+    mine[0] += n * (quanta + kI4Start);
     mine[1] += n * ((quanta + (1 << kI4PieceShift) - 1) >> kI4PieceShift);
   }
   int incl[2] = {mine[0], mine[1]};
@@ -232,18 +235,20 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     }
   }
   const bool few = totals[1] <= workers;
-  const int shift = few ? kI4PieceShift : 0;  // log2 of a piece's quanta
-  auto pieces_of = [&](int quanta) { return (quanta + (1 << shift) - 1) >> shift; };
+  // Segments lie end to end in units: pieces of four quanta, or single quanta behind kI4Start units for what a run costs besides
+  auto units_of = [&](int quanta) { return few ? (quanta + (1 << kI4PieceShift) - 1) >> kI4PieceShift : quanta + kI4Start; };
+  auto quantum_at = [&](int unit, int quanta) { return min(few ? unit << kI4PieceShift : max(unit - kI4Start, 0), quanta); };
+  const int start = few ? 0 : kI4Start;
   const int total = few ? totals[1] : totals[0], held_here = few ? mine[1] : mine[0], excl = few ? before[1] + incl[1] - mine[1] : before[0] + incl[0] - mine[0];
   const int per = (total + workers - 1) / workers;
-  // where each group starts: the thread whose sequences hold that piece says so
+  // where each group starts: the thread whose sequences hold that unit says so
   for (int k = 0; k < C::WARPS >> gsh; k++) {
     const int s0 = ((int)blockIdx.x * (C::WARPS >> gsh) + k) * per;
     if (s0 < total && excl <= s0 && s0 < excl + held_here) {
       int acc = excl;
       for (int b = b_lo; b < b_hi; b++) {
         const I4Seq s = i4_seq(p, b, ROWS);
-        const int n = pieces_of(quanta_of(s.pages)) * s.chunks * p.c.Nkv;
+        const int n = units_of(quanta_of(s.pages)) * s.chunks * p.c.Nkv;
         if (s0 < acc + n) {
           start_b[k] = b;
           start_off[k] = s0 - acc;
@@ -259,15 +264,15 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 
   // ---- the share as runs: parts of one segment each
   struct Run {
-    int b, n, chunk, seg0;     // sequence (-1: none left), key head, row chunk, first piece of the segment among all pieces
-    int qi, qend, left;        // quanta of the segment, pieces of the share behind this run
+    int b, n, chunk, seg0;     // sequence (-1: none left), key head, row chunk, first unit of the segment
+    int qi, qend, left;        // quanta of the segment, units of the share behind this run
     int keys, quanta, chunks;  // of the sequence
   };
-  auto clip = [&](Run& r, int piece) {  // the run starts at that piece of the segment
-    const int take = min(pieces_of(r.quanta) - piece, r.left);
+  auto clip = [&](Run& r, int unit) {  // the run starts at that unit of the segment
+    const int take = min(units_of(r.quanta) - unit, r.left);
     r.left -= take;
-    r.qi = piece << shift;
-    r.qend = min(r.quanta, (piece + take) << shift);
+    r.qi = quantum_at(unit, r.quanta);
+    r.qend = quantum_at(unit + take, r.quanta);
   };
   auto enter = [&](Run& r) {
     const I4Seq s = i4_seq(p, r.b, ROWS);
@@ -276,36 +281,39 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     r.chunks = s.chunks;
   };
   auto next = [&](Run& r) {
-    if (r.left == 0) {
-      r.b = -1;
-      return;
-    }
-    r.seg0 += pieces_of(r.quanta);
-    if (++r.chunk == r.chunks) {
-      r.chunk = 0;
-      if (++r.n == p.c.Nkv) {
-        r.n = 0;
-        do {
-          if (++r.b >= p.c.B) {
-            r.b = -1;
-            return;
-          }
-          enter(r);
-        } while (r.quanta * r.chunks == 0);
+    do {
+      if (r.left == 0) {
+        r.b = -1;
+        return;
       }
-    }
-    clip(r, 0);
+      r.seg0 += units_of(r.quanta);
+      if (++r.chunk == r.chunks) {
+        r.chunk = 0;
+        if (++r.n == p.c.Nkv) {
+          r.n = 0;
+          do {
+            if (++r.b >= p.c.B) {
+              r.b = -1;
+              return;
+            }
+            enter(r);
+          } while (r.quanta * r.chunks == 0);
+        }
+      }
+      clip(r, 0);
+    } while (r.qi == r.qend);
   };
   Run now;
   {
     now.b = start_b[grp];
     enter(now);
-    const int pieces = pieces_of(now.quanta), at = start_off[grp], segment = at / pieces, piece = at % pieces;
+    const int units = units_of(now.quanta), at = start_off[grp], segment = at / units, unit = at % units;
     now.n = segment / now.chunks;
     now.chunk = segment % now.chunks;
-    now.seg0 = q0 - piece;
+    now.seg0 = q0 - unit;
     now.left = q1 - q0;
-    clip(now, piece);
+    clip(now, unit);
+    if (now.qi == now.qend) next(now);
   }
 
   unsigned char* base = i4_smem + warp * C::WARP_BYTES;
@@ -357,7 +365,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   int stage = 0;
   for (; now.b >= 0; next(now)) {
     const int n_tok = i4_seq(p, now.b, ROWS).n, tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
-    const int w0 = now.seg0 / per, w1 = (now.seg0 + pieces_of(now.quanta) - 1) / per;  // the groups that share the segment
+    const int w0 = (now.seg0 + start) / per, w1 = (now.seg0 + units_of(now.quanta) - 1) / per;  // the groups that share the segment
     const bool whole = w0 == w1;
     unsigned long long word_was = 0;
     if (!whole && gtid == 0) word_was = *reinterpret_cast<volatile unsigned long long*>(p.counters + w0);
@@ -639,7 +647,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     // ---- the run's end: rows of (maximum, sum, output); a lane has 8 dimensions 64 h + 8 g + .. of the rows 4 j + t
     const int rows = min(ROWS, n_tok * p.R - now.chunk * ROWS);
     // A part is [RT][G][2][32 lanes] float4 as the lanes have them, then maxima and sums; one of a share's first, one of its last segment
-    auto part_of = [&](int k) { return p.part + ((int64_t)k * 2 + (now.seg0 < k * per ? 0 : 1)) * ROWS * (H + 2); };
+    auto part_of = [&](int k) { return p.part + ((int64_t)k * 2 + (now.seg0 + start < k * per ? 0 : 1)) * ROWS * (H + 2); };
     auto row_out = [&](int r) {
       const int row = now.chunk * ROWS + r;
       return p.out + ((int64_t)(tok0 + row / p.R) * p.Nq + now.n * p.R + row % p.R) * H;
