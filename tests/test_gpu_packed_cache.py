@@ -227,11 +227,11 @@ def check_attention(cache, q, out, old, new, cu, causal, scale, rows=None):
         kc, ks, kz, vc, vs, vz = sequence_heads(cache, b, m + n)
         x = q[at:at + n].double()
         want, w = U.attention(x, kz + kc * ks, vz + vc * vs, m, causal, scale)
-        # scores: q as whole numbers of 2^-19 of its row's largest value (half a step off at most, times a code of up to 15 and its
-        # scale), then some ten roundings of sums and products in fp32
+        # scores: q as whole numbers of 2^-17 of its row's largest value or finer (half a step off at most, times a code of up to 15 and
+        # its scale), then some ten roundings of sums and products in fp32
         size = torch.einsum("nhd,mhd->hnm", x.abs(), (kz.abs() + 15 * ks).repeat_interleave(R, 1)) * abs(scale)
         steps = x.abs().amax(-1).T[..., None] * (15 * ks).repeat_interleave(R, 1).sum(-1).T[:, None] * abs(scale)
-        delta = (16 * 2.0 ** -24 * size + 2.0 ** -20 * steps).amax(-1)                 # [heads, n]
+        delta = (16 * 2.0 ** -24 * size + 2.0 ** -18 * steps).amax(-1)                 # [heads, n]
         rounded = torch.einsum("hnm,mhd->nhd", w, (vs * (vc - 8).abs()).repeat_interleave(R, 1))  # weights times scales are rounded
         plain = torch.einsum("hnm,mhd->nhd", w, (vz.abs() + 8 * vs + vs * vc).repeat_interleave(R, 1))
         # sums in fp32 over the keys, weights off by their scores' error and that of the exponential (2^-22)

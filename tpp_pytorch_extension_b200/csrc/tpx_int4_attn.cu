@@ -5,12 +5,16 @@
 // The loop over the cache is bound by instructions per code, not by the matrix unit, so codes go to mma.sync as nearly as they lie there,
 // scales and minima around them (tcgen05 has no form this narrow: it would need 128 query rows or keys):
 //   q.K  = sum over groups of 64:  ks (q . kc) + kz sum(q)
-//          m16n8k32 u8 x s8: two ANDs and a shift turn eight codes into bytes. q is a 20-bit integer per value times a power of two per
-//          row, cut into three digits of 7 bits, each a column: exact products, and sums exact in 32 bits. Columns (2 r, 2 r + 1) are
-//          the upper digits of row r, so that a lane has whole scores; the accumulator starts at the bits of 1.5 * 2^23, which makes it a float.
+//          m16n8k32 u8 x s8 on the bytes as they lie: a byte is 16 odd + even, and
+//          q_even even + q_odd odd = (q_odd / 16) byte + (q_even - q_odd / 16) (byte & 15), so eight codes cost one AND. The two
+//          factors are whole numbers of 2^-21 of the row's largest value (q_odd: 2^-17), cut into three signed digits of 8 bits, each a
+//          column: products and sums are exact in 32 bits. Columns (2 r, 2 r + 1) are the upper digits of row r, so that a lane has
+//          whole scores; the accumulator starts at the bits of 1.5 * 2^23, which makes it a float.
 //   P V  = sum over t: (p vs) (vc - 8) + p (vz + 8 vs)
-//          m16n8k16 fp16: codes become fp16 by two ANDs and one HFMA2 per pair; centred, since p vs is rounded to fp16 and that should not be weighed with
-//          the range's offset. vs is taken relative to a power of two that follows the largest scale seen, which keeps p vs in fp16's range.
+//          m16n8k16 fp16: a byte of two codes in the mantissa of 1024 is an fp16, and so is its lower code alone; both go to the matrix unit
+//          centred (one addition per pair) and the upper code's sum is the difference / 16. Centred, since p vs is rounded to fp16 and that
+//          should not be weighed with the range's offset. vs is taken relative to a power of two that follows the largest scale seen,
+//          which keeps p vs in fp16's range.
 // The cache is the 16-row operand: 16 tokens for keys, 16 of the head's dimensions for values. Weights get to the second product by movmatrix.
 //
 // A page of a head (4608 bytes at H = 128) is one warp's work item, fetched by cp.async into a ring of the warp's own: no barrier in the
@@ -76,14 +80,17 @@ __device__ __forceinline__ uint32_t i4_pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float i4_pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-// The codes in bits 0..3 (SHIFT 0) or 4..7 (SHIFT 4) of both halves of a word, minus 8, as fp16: 1024 + code << SHIFT is an fp16 as it stands
-template <int SHIFT>
-__device__ __forceinline__ uint32_t i4_centred(uint32_t w) {
-  const uint32_t v = (w & (0x000f000fu << SHIFT)) | 0x64006400u;
+__device__ __forceinline__ uint32_t i4_add_f16(uint32_t a, uint32_t b) {
   uint32_t r;
-  if (SHIFT == 0) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0xe408e408u));                        // -1032
-  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0x2c002c00u), "r"(0xd480d480u));              // / 16, - 72
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+// Two codes of two keys: the bytes B (0: bits 0..7, 1: bits 8..15) of both halves of w, minus 136, and their lower codes, minus 8, as fp16
+template <int B>
+__device__ __forceinline__ void i4_centred(uint32_t w, uint32_t& both, uint32_t& lower) {
+  const uint32_t v = __byte_perm(w, 0x64646464u, B == 0 ? 0x4240 : 0x4341);  // 1024 + byte
+  both = i4_add_f16(v, 0xe488e488u);                                        // - 1160
+  lower = i4_add_f16(v & 0xff0fff0fu, 0xe408e408u);                         // - 1032
 }
 __device__ __forceinline__ void i4_cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -397,22 +404,27 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
           if (o < 8) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // within a group of 64
         }
         const float other = __shfl_xor_sync(0xffffffffu, sum, LR / 2);
-        // top * 2^k in [2^19, 2^20): Q = hi 2^14 + mid 2^7 + lo, -64 <= hi < 64, 0 <= mid, lo < 128, read off the bits of 1.5 * 2^23 + Q
-        const int k = min(19 - ((int)((__float_as_uint(top) >> 23) & 255) - 127), 120);
-        const float up = i4_pow2(k);
-        uint32_t d[3][2];  // digits: bytes of the even and of the odd values
-#pragma unroll
-        for (int odd = 0; odd < 2; odd++) {
-          uint32_t b[4];   // digits of a value in its bytes 0..2
+        const int k = min(21 - ((int)((__float_as_uint(top) >> 23) & 255) - 127), 120);  // top * 2^k in [2^21, 2^22)
+        const float up = i4_pow2(k), up16 = i4_pow2(k - 4);
+        uint32_t d[3][2];  // digits: bytes of the factors of (byte & 15), of the whole byte
+        {
+          uint32_t e[4], f[4];
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t Q = __float_as_uint(fmaf(x[2 * i + odd], up, __uint_as_float(kI4Magic)));
-            b[i] = (Q & 0x7fu) | ((Q << 1) & 0x7f00u) | ((Q << 2) & 0xff0000u);
+            const uint32_t Qo = __float_as_uint(fmaf(x[2 * i + 1], up16, __uint_as_float(kI4Magic)));
+            const uint32_t Qe = __float_as_uint(fmaf(x[2 * i], up, __uint_as_float(kI4Magic)));
+            // bytes 0..2 become signed digits, the lowest first
+            e[i] = (Qe - Qo + 0x8080u) ^ 0x8080u;
+            f[i] = (Qo - kI4Magic + 0x8080u) ^ 0x8080u;
           }
-          const uint32_t p01 = __byte_perm(b[0], b[1], 0x5140), p23 = __byte_perm(b[2], b[3], 0x5140);
-          d[2][odd] = __byte_perm(p01, p23, 0x5410);
-          d[1][odd] = __byte_perm(p01, p23, 0x7632);
-          d[0][odd] = __byte_perm(__byte_perm(b[0], b[1], 0x0062), __byte_perm(b[2], b[3], 0x0062), 0x5410);
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const uint32_t* b = half ? f : e;
+            const uint32_t p01 = __byte_perm(b[0], b[1], 0x5140), p23 = __byte_perm(b[2], b[3], 0x5140);
+            d[2][half] = __byte_perm(p01, p23, 0x5410);
+            d[1][half] = __byte_perm(p01, p23, 0x7632);
+            d[0][half] = __byte_perm(__byte_perm(b[0], b[1], 0x0062), __byte_perm(b[2], b[3], 0x0062), 0x5410);
+          }
         }
         const float bad = top * 0.0f;  // a NaN where any value is not finite
         if (r < ROWS) {
@@ -479,11 +491,11 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const uint32_t a = kw[0][2 * h + i], b = kw[1][2 * h + i];
-            const uint32_t a0 = a & 0x0f0f0f0fu, a1 = b & 0x0f0f0f0fu, a2 = (a >> 4) & 0x0f0f0f0fu, a3 = (b >> 4) & 0x0f0f0f0fu;
+            const uint32_t a0 = a & 0x0f0f0f0fu, a1 = b & 0x0f0f0f0fu;
 #pragma unroll
             for (int n = 0; n < C::TILES; n++) {
-              if (i == 0) i4_mma_first(d[n], a0, a1, a2, a3, qf[n][2 * h]);
-              else i4_mma_u8(d[n], a0, a1, a2, a3, qf[n][2 * h + 1]);
+              if (i == 0) i4_mma_first(d[n], a0, a1, a, b, qf[n][2 * h]);
+              else i4_mma_u8(d[n], a0, a1, a, b, qf[n][2 * h + 1]);
             }
           }
 #pragma unroll
@@ -491,7 +503,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
             const float s = __uint_as_float(kp[r][h] << 16), z = __uint_as_float(kp[r][h] & 0xffff0000u);
 #pragma unroll
             for (int j = 0; j < RT; j++) {
-              const float f = fmaf(fmaf(i4_count(d[j][2 * r]), 128.0f, i4_count(d[j][2 * r + 1])), 128.0f, i4_count(d[RT + j / 2][2 * r + (j & 1)]));
+              const float f = fmaf(fmaf(i4_count(d[j][2 * r]), 256.0f, i4_count(d[j][2 * r + 1])), 256.0f, i4_count(d[RT + j / 2][2 * r + (j & 1)]));
               x[j][m][r] = fmaf(s * qsc[j], f, h == 0 ? z * qs[j][0] : fmaf(z, qs[j][h], x[j][m][r]));
             }
           }
@@ -615,22 +627,25 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 #pragma unroll
         for (int h = 0; h < G; h++) {
           // low halves: dimensions 64 h + 8 g + 0..3 of the keys t and t + 4, high halves: + 4..7
-          uint32_t xa = __byte_perm(va[h], va[G + h], 0x5410), ya = __byte_perm(va[h], va[G + h], 0x7632);
-          uint32_t xb = __byte_perm(vb[h], vb[G + h], 0x5410), yb = __byte_perm(vb[h], vb[G + h], 0x7632);
+          const uint32_t xa = __byte_perm(va[h], va[G + h], 0x5410), ya = __byte_perm(va[h], va[G + h], 0x7632);
+          const uint32_t xb = __byte_perm(vb[h], vb[G + h], 0x5410), yb = __byte_perm(vb[h], vb[G + h], 0x7632);
+          uint32_t f[2][8];  // [codes 2 i + 1 with 2 i, codes 2 i alone]: i = 0, 1
+          i4_centred<0>(xa, f[1][0], f[0][0]);
+          i4_centred<0>(ya, f[1][1], f[0][1]);
+          i4_centred<0>(xb, f[1][2], f[0][2]);
+          i4_centred<0>(yb, f[1][3], f[0][3]);
+          i4_centred<1>(xa, f[1][4], f[0][4]);
+          i4_centred<1>(ya, f[1][5], f[0][5]);
+          i4_centred<1>(xb, f[1][6], f[0][6]);
+          i4_centred<1>(yb, f[1][7], f[0][7]);
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const uint32_t f0 = i4_centred<0>(xa), f1 = i4_centred<0>(ya), f2 = i4_centred<0>(xb), f3 = i4_centred<0>(yb);
-            const uint32_t f4 = i4_centred<4>(xa), f5 = i4_centred<4>(ya), f6 = i4_centred<4>(xb), f7 = i4_centred<4>(yb);
+          for (int v = 0; v < VT; v++) {
+            const uint32_t(&b)[2] = pb[v][RT == 1 ? 0 : h];
 #pragma unroll
-            for (int v = 0; v < VT; v++) {
-              const uint32_t(&b)[2] = pb[v][RT == 1 ? 0 : h];
-              i4_mma_f16(acc[v][h][i], f0, f1, f2, f3, b[0], b[1]);
-              i4_mma_f16(acc[v][h][i + 1], f4, f5, f6, f7, b[0], b[1]);
+            for (int i = 0; i < 4; i++) {
+              const uint32_t* a = &f[i & 1][(i >> 1) * 4];
+              i4_mma_f16(acc[v][h][i], a[0], a[1], a[2], a[3], b[0], b[1]);
             }
-            xa >>= 8;
-            ya >>= 8;
-            xb >>= 8;
-            yb >>= 8;
           }
         }
       }
@@ -666,9 +681,10 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 #pragma unroll
         for (int h = 0; h < G; h++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            o[j][h][i] = fmaf(acc[j / 2][h][i][RT == 1 ? h : j & 1], up, zacc[j][h]);
-            o[j][h][4 + i] = fmaf(acc[j / 2][h][i][2 + (RT == 1 ? h : j & 1)], up, zacc[j][h]);
+          for (int i = 0; i < 8; i++) {
+            const int c = i & 3, e = (RT == 1 ? h : j & 1) + 2 * (i >> 2);  // accumulators c odd hold 16 times their code's sum and that of c - 1
+            const float sum = c & 1 ? (acc[j / 2][h][c][e] - acc[j / 2][h][c - 1][e]) * 0.0625f : acc[j / 2][h][c][e];
+            o[j][h][i] = fmaf(sum, up, zacc[j][h]);
           }
       }
     }
