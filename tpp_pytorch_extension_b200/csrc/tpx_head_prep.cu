@@ -6,7 +6,8 @@
 // per 64 cached values: bound by HBM for prompts, by the launch and one chain of dependent loads for single tokens.
 //
 // H / 16 lanes share a head (two pieces of 8 values per lane, which are the two halves of its rotary pairs), so that norms and ranges
-// of 64 values are a few shuffles. A thread does UNITS heads of one token: their loads go out together and share its cosines and sines.
+// of 64 values are a few shuffles. A warp works on heads of one kind of one token: a thread does up to UNITS of them, whose loads go out
+// together, with the products of norm weights, cosines and sines kept in registers.
 #include "tpx_int4.cuh"
 
 namespace tpx {
@@ -20,7 +21,7 @@ struct PrepParams {
   uint16_t *q_out, *k_out;
   I4Cache c;
   int64_t ldq, ldk, ldv, max_pos, ld_ep;
-  int T, Nq, Nkv, H, rot, per_token;  // per_token: threads per token
+  int T, Nq, Nkv, H, rot, wq, wkv, wpt;  // warps per token for queries, for keys and for values each, in all
   float eps;
   int norm_f32, cached;
 };
@@ -87,7 +88,7 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
   }
   if (!dst) return;
   uint32_t param[2];
-  float least[2], step[2];  // halves of minimum and scale: the range of a row may pass the largest float
+  float least[2], step[2], back[2];  // halves of minimum and scale: the range of a row may pass the largest float
 #pragma unroll
   for (int g = 0; g < 2; g++) {
     const uint32_t a = g ? mn & 0xffff0000u : mn << 16, b = g ? mx & 0xffff0000u : mx << 16;
@@ -96,6 +97,7 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
     const bool fine = (a & 0x7f800000u) != 0x7f800000u && (b & 0x7f800000u) != 0x7f800000u;
     const uint32_t s = fine ? f32_to_bf16_bits(__fdiv_rn(half_range, 7.5f)) : 0x7fc0u;
     step[g] = 0.5f * __uint_as_float(s << 16);
+    back[g] = __frcp_rn(step[g]);
     param[g] = s | (fine ? a & 0xffff0000u : 0x7fc00000u);
   }
   uint32_t* codes = reinterpret_cast<uint32_t*>(dst + (is_v ? H / 2 * kI4Page + H / kI4Group * 4 * kI4Page : 0));
@@ -105,10 +107,18 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
     const int d = half ? dhi : dlo, g = half ? gh : gl;
     float x[8];
     prep_unpack(half ? hi : lo, x);
-    const float base = g ? least[1] : least[0], s = g ? step[1] : step[0];
+    const float base = g ? least[1] : least[0], s = g ? step[1] : step[0], y = g ? back[1] : back[0];
     uint32_t word = 0;
-    if (s > 0.0f) {
+    if (s > 1e-30f && s < 1e30f) {
+      // The quotient with its remainder taken back in is the rounded one, as a division's would be, ties exact; 1.5 * 2^23 rounds it to a whole number
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
+      for (int i = 7; i >= 0; i--) {
+        const float v = fmaf(0.5f, x[i], -base), q = v * y, r = fmaf(fmaf(-q, s, v), y, q);
+        sum[i >> 2] = fmaf(sum[i >> 2], 16.0f, fminf((r + 12582912.0f) - 12582912.0f, 15.0f));
+      }
+      word = (__float_as_uint(sum[0] + 12582912.0f) & 0xffffu) | __float_as_uint(sum[1] + 12582912.0f) << 16;
+    } else if (s > 0.0f) {
       for (int i = 0; i < 8; i++) word |= (uint32_t)fminf(rintf(__fdiv_rn(fmaf(0.5f, x[i], -base), s)), 15.0f) << (4 * i);
     }
     codes[is_v ? i4_v_word(H, t, d) : i4_k_word(H, t, d)] = word;
@@ -117,135 +127,201 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
     for (int g = 0; g < H / kI4Group; g++) params[g] = param[g];
 }
 
+// Pairs of fp32 in one operation
+__device__ __forceinline__ float2 prep_fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{ .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 prep_mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{ .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w; }"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ void prep_pairs(uint4 v, float2 (&x)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) x[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 prep_pack(const float2 (&x)[4]) {
+  const float f[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+  return prep_pack(f);
+}
+
 template <int LANES, int UNITS>
-__global__ void head_prep_kernel(PrepParams p) {
+__global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
   pdl_trigger();
   pdl_wait();
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int row = (int)(idx / p.per_token), in_row = (int)(idx % p.per_token);
-  const int sub = in_row % LANES, first = in_row / LANES, groups = p.per_token / LANES;
-  const int heads = p.Nq + p.Nkv + (p.cached ? p.Nkv : 0);
-  const bool live_lane = sub * 16 < p.H && row < p.T;  // head sizes that are no power of two leave lanes idle
+  const int warp = (int)(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+  const int row = warp / p.wpt, in_row = warp % p.wpt;
+  if (row >= p.T) return;  // a warp as a whole
+  const int kind = in_row < p.wq ? 0 : in_row < p.wq + p.wkv ? 1 : 2;  // queries, keys, values
+  const int N = kind ? p.Nkv : p.Nq, groups = (kind ? p.wkv : p.wq) * (32 / LANES);
+  const int sub = lane % LANES, first = (in_row - (kind == 0 ? 0 : kind == 1 ? p.wq : p.wq + p.wkv)) * (32 / LANES) + lane / LANES;
+  const bool live_lane = sub * 16 < p.H;  // head sizes that are no power of two leave lanes idle
   // a lane's pieces: the first rot / 16 lanes hold rotary pairs, the others two pieces side by side
   const bool turns = sub * 16 < p.rot;
   const int dlo = turns ? sub * 8 : sub * 16, dhi = turns ? dlo + p.rot / 2 : dlo + 8;
 
+  const uint16_t* src = kind == 0 ? p.q + row * p.ldq : kind == 1 ? p.k + row * p.ldk : p.v + row * p.ldv;
   uint4 lo[UNITS], hi[UNITS];
 #pragma unroll
   for (int u = 0; u < UNITS; u++) {
     const int h = first + u * groups;
     lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-    if (live_lane && h < heads) {
-      const uint16_t* src = h < p.Nq ? p.q + row * p.ldq + h * p.H
-                                     : h < p.Nq + p.Nkv ? p.k + row * p.ldk + (h - p.Nq) * p.H : p.v + row * p.ldv + (h - p.Nq - p.Nkv) * p.H;
-      lo[u] = *reinterpret_cast<const uint4*>(src + dlo);
-      hi[u] = *reinterpret_cast<const uint4*>(src + dhi);
+    if (live_lane && h < N) {
+      lo[u] = *reinterpret_cast<const uint4*>(src + h * p.H + dlo);
+      hi[u] = *reinterpret_cast<const uint4*>(src + h * p.H + dhi);
     }
   }
   int seq = -1;
   int64_t place = 0;
-  const bool placed = p.cached || p.cu;
-  if (row < p.T && placed) {
+  if (p.cached) {
     seq = i4_sequence(p.cu, p.c.B, row);
-    if (seq >= 0 && p.cached) place = (int64_t)max(p.c.lengths[seq], 0) + (p.cu ? row - p.cu[seq] : 0);
+    if (seq < 0) return;  // a row of no sequence: the warp as a whole
+    place = (int64_t)max(p.c.lengths[seq], 0) + (p.cu ? row - p.cu[seq] : 0);
   }
-  const bool live = row < p.T && (!placed || seq >= 0);
-  float cs[8], sn[8];
-  bool rotate = turns && live && p.ep;
+  const void* norm = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
+  bool rotate = turns && kind < 2;
+  int64_t pos = 0;
   if (rotate) {
-    const int64_t pos = p.pos ? p.pos[row] : place;
+    pos = p.pos ? p.pos[row] : place;
     rotate = pos >= 0 && pos < p.max_pos;
+  }
+  // out_lo = x_lo (w_lo c) - x_hi (w_hi s), out_hi = x_hi (w_hi c) + x_lo (w_lo s)
+  float2 lc[4], hs[4], hc[4], ls[4];
+  if (kind < 2) {
+    float wl[8], wh[8], cs[8], sn[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      wl[i] = wh[i] = cs[i] = 1.0f;
+      sn[i] = 0.0f;
+    }
+    if (norm && live_lane) {
+      prep_weights(norm, p.norm_f32, dlo, wl);
+      prep_weights(norm, p.norm_f32, dhi, wh);
+    }
     if (rotate) {
       prep_weights(p.ep + pos * p.ld_ep, 1, dlo, cs);
       prep_weights(p.ep + (p.max_pos + pos) * p.ld_ep, 1, dlo, sn);
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      lc[i] = make_float2(wl[2 * i] * cs[2 * i], wl[2 * i + 1] * cs[2 * i + 1]);
+      hs[i] = make_float2(-wh[2 * i] * sn[2 * i], -wh[2 * i + 1] * sn[2 * i + 1]);
+      hc[i] = make_float2(wh[2 * i] * cs[2 * i], wh[2 * i + 1] * cs[2 * i + 1]);
+      ls[i] = make_float2(wl[2 * i] * sn[2 * i], wl[2 * i + 1] * sn[2 * i + 1]);
+    }
   }
 #pragma unroll
   for (int u = 0; u < UNITS; u++) {
+    if (u * groups >= N) break;
     const int h = first + u * groups;
-    const bool is_q = h < p.Nq, is_v = h >= p.Nq + p.Nkv;
-    const void* norm = is_q ? p.q_norm : p.k_norm;
-    float a[8], b[8];
-    prep_unpack(lo[u], a);
-    prep_unpack(hi[u], b);
-    float ss = 0.0f;
+    const bool write = live_lane && h < N;
+    if (kind < 2) {
+      float2 a[4], b[4];
+      prep_pairs(lo[u], a);
+      prep_pairs(hi[u], b);
+      if (norm) {
+        float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) ss += a[i] * a[i] + b[i] * b[i];
+        for (int i = 0; i < 4; i++) s2 = prep_fma2(b[i], b[i], prep_fma2(a[i], a[i], s2));
+        float ss = s2.x + s2.y;
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!is_v && (norm || rotate)) {
-      if (norm && live_lane) {
-        const float inv = 1.0f / sqrtf(ss / (float)p.H + p.eps);
-        float g[8];
-        prep_weights(norm, p.norm_f32, dlo, g);
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss / (float)p.H + p.eps);
+        const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 8; i++) a[i] = a[i] * inv * g[i];
-        prep_weights(norm, p.norm_f32, dhi, g);
-#pragma unroll
-        for (int i = 0; i < 8; i++) b[i] = b[i] * inv * g[i];
-      }
-      if (rotate) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float x = a[i], y = b[i];
-          a[i] = x * cs[i] - y * sn[i];
-          b[i] = y * cs[i] + x * sn[i];
+        for (int i = 0; i < 4; i++) {
+          a[i] = prep_mul2(a[i], inv2);
+          b[i] = prep_mul2(b[i], inv2);
         }
       }
-      lo[u] = prep_pack(a);
-      hi[u] = prep_pack(b);
-    }
-    const bool write = live && live_lane && h < heads;
-    uint16_t* out = is_q ? p.q_out : is_v ? nullptr : p.k_out;
-    if (write && out) {
-      out += is_q ? ((int64_t)row * p.Nq + h) * p.H : ((int64_t)row * p.Nkv + h - p.Nq) * p.H;
-      *reinterpret_cast<uint4*>(out + dlo) = lo[u];
-      *reinterpret_cast<uint4*>(out + dhi) = hi[u];
+      if (norm || rotate) {
+        float2 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          x[i] = prep_mul2(a[i], lc[i]);
+          y[i] = prep_mul2(b[i], hc[i]);
+          if (rotate) {
+            x[i] = prep_fma2(b[i], hs[i], x[i]);
+            y[i] = prep_fma2(a[i], ls[i], y[i]);
+          }
+        }
+        lo[u] = prep_pack(x);
+        hi[u] = prep_pack(y);
+      }
+      uint16_t* out = kind == 0 ? p.q_out : p.k_out;
+      if (write && out) {
+        out += ((int64_t)row * N + h) * p.H;
+        *reinterpret_cast<uint4*>(out + dlo) = lo[u];
+        *reinterpret_cast<uint4*>(out + dhi) = hi[u];
+      }
     }
     if (LANES == 4 || LANES == 8) {  // the head sizes of the cache
-      // the whole warp takes part in the ranges' shuffles
-      if (p.cached && __any_sync(0xffffffffu, write && !is_q)) {
-        const int n = is_v ? h - p.Nq - p.Nkv : h - p.Nq;
-        uint8_t* dst = write && !is_q ? i4_head(p.c, seq, place, n, 36 * p.H) : nullptr;
-        prep_to_cache<LANES>(dst, (int)(place % kI4Page), is_v, p.H, dlo, dhi, lo[u], hi[u], sub);
-      }
+      if (p.cached && kind > 0)      // the whole warp takes part in the ranges' shuffles
+        prep_to_cache<LANES>(write ? i4_head(p.c, seq, place, h, 36 * p.H) : nullptr, (int)(place % kI4Page), kind == 2, p.H, dlo, dhi, lo[u], hi[u], sub);
     }
   }
 }
 
-template <int H>
-__global__ void int4_read_kernel(I4Cache c, const int32_t* __restrict__ cu, int T, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out) {
+// A thread has one piece of 8 values of up to UNITS heads of a token: where the token is found once, and the loads go out together.
+template <int H, int UNITS>
+__global__ void __launch_bounds__(256) int4_read_kernel(I4Cache c, const int32_t* __restrict__ cu, int T, int groups, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out) {
   pdl_trigger();
   pdl_wait();
+  using L = I4<H>;
   constexpr int PIECES = H / 8;
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int d = (int)(idx % PIECES) * 8;
   const int64_t rest = idx / PIECES;
-  const int n = (int)(rest % c.Nkv);
-  const int64_t row = rest / c.Nkv;
+  const int first = (int)(rest % groups);
+  const int64_t row = rest / groups;
   if (row >= T) return;
   const int seq = i4_sequence(cu, c.B, (int)row);
   if (seq < 0) return;
   const int64_t place = (int64_t)max(c.lengths[seq], 0) + (cu ? (int)row - cu[seq] : 0);
-  const uint8_t* src = i4_head(c, seq, place, n, I4<H>::BYTES);
   const int t = (int)(place % kI4Page);
+  const uint8_t* page = i4_head(c, seq, place, 0, L::BYTES);
+  uint32_t word[UNITS][2], param[UNITS][2];
 #pragma unroll
-  for (int is_v = 0; is_v < 2; is_v++) {
-    uint16_t* out = is_v ? v_out : k_out;
-    if (!out) continue;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (src) {
-      const uint8_t* codes = src + (is_v ? I4<H>::VC : I4<H>::KC);
-      const uint32_t word = reinterpret_cast<const uint32_t*>(codes)[is_v ? i4_v_word(H, t, d) : i4_k_word(H, t, d)];
-      const uint32_t param = reinterpret_cast<const uint32_t*>(codes + I4<H>::CODES)[t * I4<H>::G + d / kI4Group];
-      const float s = __uint_as_float(param << 16), z = __uint_as_float(param & 0xffff0000u);
+  for (int u = 0; u < UNITS; u++)
+#pragma unroll
+    for (int is_v = 0; is_v < 2; is_v++) {
+      word[u][is_v] = param[u][is_v] = 0;
+      if (page && first + u * groups < c.Nkv) {
+        const uint8_t* codes = page + (int64_t)(first + u * groups) * L::BYTES + (is_v ? L::VC : L::KC);
+        word[u][is_v] = reinterpret_cast<const uint32_t*>(codes)[is_v ? i4_v_word(H, t, d) : i4_k_word(H, t, d)];
+        param[u][is_v] = reinterpret_cast<const uint32_t*>(codes + L::CODES)[t * L::G + d / kI4Group];
+      }
+    }
+#pragma unroll
+  for (int u = 0; u < UNITS; u++)
+#pragma unroll
+    for (int is_v = 0; is_v < 2; is_v++) {
+      uint16_t* out = is_v ? v_out : k_out;
+      if (!out || first + u * groups >= c.Nkv) continue;
+      const float s = __uint_as_float(param[u][is_v] << 16), z = __uint_as_float(param[u][is_v] & 0xffff0000u);
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = fmaf((float)(word >> (4 * i) & 15), s, z);
-      w = prep_pack(x);
+      for (int i = 0; i < 8; i++) x[i] = fmaf((float)(word[u][is_v] >> (4 * i) & 15), s, z);
+      *reinterpret_cast<uint4*>(out + (row * c.Nkv + first + u * groups) * H + d) = prep_pack(x);
     }
-    *reinterpret_cast<uint4*>(out + ((int64_t)row * c.Nkv + n) * H + d) = w;
-  }
+}
+
+template <int H>
+static int read_launch(const I4Cache& c, const int32_t* cu, int T, uint16_t* k_out, uint16_t* v_out, cudaStream_t st) {
+  const bool many = (int64_t)T * c.Nkv * (H / 8) >= (int64_t)sm_count() * 2048;
+  const int units = many ? 4 : 1, groups = (c.Nkv + units - 1) / units;
+  const int64_t grid = ((int64_t)T * groups * (H / 8) + 255) / 256;
+  TPX_REQUIRE(grid < (1ll << 31), TPX_ERR_UNSUPPORTED, "int4_read: too many tokens in one call");
+  TPX_CUDA_OK(many ? launch_pdl(int4_read_kernel<H, 4>, dim3((unsigned)grid), dim3(256), 0, st, c, cu, T, groups, k_out, v_out)
+                   : launch_pdl(int4_read_kernel<H, 1>, dim3((unsigned)grid), dim3(256), 0, st, c, cu, T, groups, k_out, v_out));
+  return TPX_OK;
 }
 
 int i4_cache_of(const TpxInt4Cache* a, I4Cache* c) {
@@ -262,13 +338,15 @@ int i4_cache_of(const TpxInt4Cache* a, I4Cache* c) {
 
 template <int LANES>
 static int prep_launch(PrepParams& p, cudaStream_t st) {
-  const int heads = p.Nq + p.Nkv + (p.cached ? p.Nkv : 0);
   // Four heads per thread once that still fills the GPU
+  const int heads = p.Nq + p.Nkv + (p.cached ? p.Nkv : 0);
   const bool many = (int64_t)p.T * heads * LANES >= (int64_t)sm_count() * 2048;
-  const int units = many ? 4 : 1, block = 256;
-  p.per_token = (heads + units - 1) / units * LANES;
-  const int64_t grid = ((int64_t)p.T * p.per_token + block - 1) / block;
-  TPX_REQUIRE(grid < (1ll << 31), TPX_ERR_UNSUPPORTED, "head_prep: too many tokens in one call");
+  const int per_warp = 32 / LANES * (many ? 4 : 1), block = 256;
+  p.wq = (p.Nq + per_warp - 1) / per_warp;
+  p.wkv = (p.Nkv + per_warp - 1) / per_warp;
+  p.wpt = p.wq + (p.cached ? 2 : 1) * p.wkv;
+  const int64_t grid = ((int64_t)p.T * p.wpt + block / 32 - 1) / (block / 32);
+  TPX_REQUIRE(grid * (block / 32) < (1ll << 31), TPX_ERR_UNSUPPORTED, "head_prep: too many tokens in one call");
   TPX_CUDA_OK(many ? launch_pdl(head_prep_kernel<LANES, 4>, dim3((unsigned)grid), dim3(block), 0, st, p)
                    : launch_pdl(head_prep_kernel<LANES, 1>, dim3((unsigned)grid), dim3(block), 0, st, p));
   return TPX_OK;
@@ -291,7 +369,7 @@ extern "C" int tpx_head_prep(const TpxHeadPrep* a, void* stream) {
                    (uintptr_t)a->k_norm | (uintptr_t)a->ep;
   TPX_REQUIRE((bits & 15) == 0 && (a->ldq | a->ldk | a->ldv) % 8 == 0, TPX_ERR_ARG, "head_prep: tensors and their rows must be 16-byte aligned");
   PrepParams p = {a->q, a->k, a->v, a->q_norm, a->k_norm, a->ep, a->pos, a->cu_seqlens, a->q_out, a->k_out, {}, a->ldq, a->ldk, a->ldv, a->max_pos, a->ld_ep,
-                  (int)a->T, (int)a->Nq, (int)a->Nkv, (int)a->H, a->ep ? (int)a->rot : 0, 0, a->eps, a->norm_is_f32, 0};
+                  (int)a->T, (int)a->Nq, (int)a->Nkv, (int)a->H, a->ep ? (int)a->rot : 0, 0, 0, 0, a->eps, a->norm_is_f32, 0};
   if (a->cache) {
     const int rc = i4_cache_of(a->cache, &p.c);
     if (rc) return rc;
@@ -317,10 +395,6 @@ extern "C" int tpx_int4_read(const TpxInt4Cache* cache, const int32_t* cu_seqlen
   TPX_REQUIRE(T >= 0 && T < (1ll << 31) && (cu_seqlens || T == cache->B), TPX_ERR_ARG, "int4_read: %ld tokens for %ld sequences", (long)T, (long)cache->B);
   TPX_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, TPX_ERR_ARG, "int4_read: outputs must be 16-byte aligned");
   if (T == 0) return TPX_OK;
-  const int64_t grid = (T * c.Nkv * (cache->H / 8) + 255) / 256;
-  TPX_REQUIRE(grid < (1ll << 31), TPX_ERR_UNSUPPORTED, "int4_read: too many tokens in one call");
-  cudaStream_t st = (cudaStream_t)stream;
-  TPX_CUDA_OK(cache->H == 128 ? launch_pdl(int4_read_kernel<128>, dim3((unsigned)grid), dim3(256), 0, st, c, cu_seqlens, (int)T, k_out, v_out)
-                              : launch_pdl(int4_read_kernel<64>, dim3((unsigned)grid), dim3(256), 0, st, c, cu_seqlens, (int)T, k_out, v_out));
-  return TPX_OK;
+  return cache->H == 128 ? read_launch<128>(c, cu_seqlens, (int)T, k_out, v_out, (cudaStream_t)stream)
+                         : read_launch<64>(c, cu_seqlens, (int)T, k_out, v_out, (cudaStream_t)stream);
 }
