@@ -8,6 +8,8 @@
 // H / 16 lanes share a head (two pieces of 8 values per lane, which are the two halves of its rotary pairs), so that norms and ranges
 // of 64 values are a few shuffles. A warp works on heads of one kind of one token: a thread does up to UNITS of them, whose loads go out
 // together, with the products of norm weights, cosines and sines kept in registers.
+#include <numeric>
+
 #include "tpx_int4.cuh"
 
 namespace tpx {
@@ -22,7 +24,8 @@ struct PrepParams {
   I4Cache c;
   int64_t ldq, ldk, ldv, max_pos, ld_ep;
   int T, Nq, Nkv, H, rot, wq, wkv, wpt;  // warps per token for queries, for keys and for values each, in all
-  float eps;
+  int stride;                                 // resident warps that walk the items
+  float eps, inv_h;
   int norm_f32, cached;
 };
 
@@ -152,63 +155,70 @@ __device__ __forceinline__ uint4 prep_pack(const float2 (&x)[4]) {
   return prep_pack(f);
 }
 
-template <int LANES, int UNITS>
-__global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
-  pdl_trigger();
-  pdl_wait();
-  const int warp = (int)(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-  const int row = warp / p.wpt, in_row = warp % p.wpt;
-  if (row >= p.T) return;  // a warp as a whole
-  const int kind = in_row < p.wq ? 0 : in_row < p.wq + p.wkv ? 1 : 2;  // queries, keys, values
-  const int N = kind ? p.Nkv : p.Nq, groups = (kind ? p.wkv : p.wq) * (32 / LANES);
-  const int sub = lane % LANES, first = (in_row - (kind == 0 ? 0 : kind == 1 ? p.wq : p.wq + p.wkv)) * (32 / LANES) + lane / LANES;
-  const bool live_lane = sub * 16 < p.H;  // head sizes that are no power of two leave lanes idle
-  // a lane's pieces: the first rot / 16 lanes hold rotary pairs, the others two pieces side by side
-  const bool turns = sub * 16 < p.rot;
-  const int dlo = turns ? sub * 8 : sub * 16, dhi = turns ? dlo + p.rot / 2 : dlo + 8;
-
-  const uint16_t* src = kind == 0 ? p.q + row * p.ldq : kind == 1 ? p.k + row * p.ldk : p.v + row * p.ldv;
-  uint4 lo[UNITS], hi[UNITS];
-#pragma unroll
-  for (int u = 0; u < UNITS; u++) {
-    const int h = first + u * groups;
-    lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-    if (live_lane && h < N) {
-      lo[u] = *reinterpret_cast<const uint4*>(src + h * p.H + dlo);
-      hi[u] = *reinterpret_cast<const uint4*>(src + h * p.H + dhi);
-    }
-  }
-  int seq = -1;
-  int64_t place = 0;
+// What a warp works on: heads of one kind of one token
+struct PrepItem {
+  int row, kind, N, groups, base;  // queries, keys, values; heads, distance of a thread's heads, the warp's first group
+  int seq;                         // -1: a row of no sequence
+  int64_t place, pos;              // of the token in the cache; pos < 0: no rotation
+};
+template <int LANES>
+__device__ __forceinline__ PrepItem prep_item(const PrepParams& p, int item) {
+  PrepItem it;
+  it.row = item / p.wpt;
+  const int in_row = item - it.row * p.wpt;
+  it.kind = in_row < p.wq ? 0 : in_row < p.wq + p.wkv ? 1 : 2;
+  it.N = it.kind ? p.Nkv : p.Nq;
+  it.groups = (it.kind ? p.wkv : p.wq) * (32 / LANES);
+  it.base = (in_row - (it.kind == 0 ? 0 : it.kind == 1 ? p.wq : p.wq + p.wkv)) * (32 / LANES);
+  it.seq = 0;
+  it.place = 0;
   if (p.cached) {
-    seq = i4_sequence(p.cu, p.c.B, row);
-    if (seq < 0) return;  // a row of no sequence: the warp as a whole
-    place = (int64_t)max(p.c.lengths[seq], 0) + (p.cu ? row - p.cu[seq] : 0);
+    it.seq = i4_sequence(p.cu, p.c.B, it.row);
+    if (it.seq >= 0) it.place = (int64_t)max(p.c.lengths[it.seq], 0) + (p.cu ? it.row - p.cu[it.seq] : 0);
   }
-  const void* norm = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-  bool rotate = turns && kind < 2;
-  int64_t pos = 0;
-  if (rotate) {
-    pos = p.pos ? p.pos[row] : place;
-    rotate = pos >= 0 && pos < p.max_pos;
-  }
+  it.pos = it.kind == 2 || p.rot == 0 ? -1 : p.pos ? p.pos[it.row] : it.place;
+  if (it.pos >= p.max_pos) it.pos = -1;
+  return it;
+}
+// A lane's pieces of a head: the first rot / 16 lanes hold rotary pairs, the others two pieces side by side
+struct PrepLane {
+  int sub, dlo, dhi;
+  bool live, turns;  // head sizes that are no power of two leave lanes idle
+};
+template <int LANES>
+__device__ __forceinline__ PrepLane prep_lane(const PrepParams& p, int lane) {
+  PrepLane l;
+  l.sub = lane % LANES;
+  l.live = l.sub * 16 < p.H;
+  l.turns = l.sub * 16 < p.rot;
+  l.dlo = l.turns ? l.sub * 8 : l.sub * 16;
+  l.dhi = l.turns ? l.dlo + p.rot / 2 : l.dlo + 8;
+  return l;
+}
+__device__ __forceinline__ const uint16_t* prep_source(const PrepParams& p, const PrepItem& it) {
+  return it.kind == 0 ? p.q + it.row * p.ldq : it.kind == 1 ? p.k + it.row * p.ldk : p.v + it.row * p.ldv;
+}
+
+// The heads of an item: load(u, lo, hi) gives the thread's pieces of its head u, angles(cs, sn) its cosines and sines
+template <int LANES, int UNITS, class Load, class Angles>
+__device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& it, const PrepLane& l, int lane, Load load, Angles angles) {
+  const void* norm = it.kind == 0 ? p.q_norm : it.kind == 1 ? p.k_norm : nullptr;
+  const bool rotate = l.turns && it.pos >= 0, turned = __all_sync(0xffffffffu, rotate || !l.live);
+  const int first = it.base + lane / LANES;
   // out_lo = x_lo (w_lo c) - x_hi (w_hi s), out_hi = x_hi (w_hi c) + x_lo (w_lo s)
   float2 lc[4], hs[4], hc[4], ls[4];
-  if (kind < 2) {
+  if (it.kind < 2) {
     float wl[8], wh[8], cs[8], sn[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       wl[i] = wh[i] = cs[i] = 1.0f;
       sn[i] = 0.0f;
     }
-    if (norm && live_lane) {
-      prep_weights(norm, p.norm_f32, dlo, wl);
-      prep_weights(norm, p.norm_f32, dhi, wh);
+    if (norm && l.live) {
+      prep_weights(norm, p.norm_f32, l.dlo, wl);
+      prep_weights(norm, p.norm_f32, l.dhi, wh);
     }
-    if (rotate) {
-      prep_weights(p.ep + pos * p.ld_ep, 1, dlo, cs);
-      prep_weights(p.ep + (p.max_pos + pos) * p.ld_ep, 1, dlo, sn);
-    }
+    if (rotate) angles(cs, sn);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       lc[i] = make_float2(wl[2 * i] * cs[2 * i], wl[2 * i + 1] * cs[2 * i + 1]);
@@ -219,13 +229,15 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
   }
 #pragma unroll
   for (int u = 0; u < UNITS; u++) {
-    if (u * groups >= N) break;
-    const int h = first + u * groups;
-    const bool write = live_lane && h < N;
-    if (kind < 2) {
+    if (u * it.groups >= it.N) break;
+    const int h = first + u * it.groups;
+    const bool write = l.live && h < it.N;
+    uint4 lo, hi;
+    load(u, lo, hi);
+    if (it.kind < 2) {
       float2 a[4], b[4];
-      prep_pairs(lo[u], a);
-      prep_pairs(hi[u], b);
+      prep_pairs(lo, a);
+      prep_pairs(hi, b);
       if (norm) {
         float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
         float ss = s2.x + s2.y;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss / (float)p.H + p.eps);
+        const float inv = rsqrtf(fmaf(ss, p.inv_h, p.eps));
         const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -241,32 +253,133 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
           b[i] = prep_mul2(b[i], inv2);
         }
       }
-      if (norm || rotate) {
+      if (norm || p.rot) {
         float2 x[4], y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           x[i] = prep_mul2(a[i], lc[i]);
           y[i] = prep_mul2(b[i], hc[i]);
-          if (rotate) {
+        }
+        if (turned || rotate) {  // the whole warp, or the lanes that do: elsewhere 0 * infinity would be added
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
             x[i] = prep_fma2(b[i], hs[i], x[i]);
             y[i] = prep_fma2(a[i], ls[i], y[i]);
           }
         }
-        lo[u] = prep_pack(x);
-        hi[u] = prep_pack(y);
+        lo = prep_pack(x);
+        hi = prep_pack(y);
       }
-      uint16_t* out = kind == 0 ? p.q_out : p.k_out;
+      uint16_t* out = it.kind == 0 ? p.q_out : p.k_out;
       if (write && out) {
-        out += ((int64_t)row * N + h) * p.H;
-        *reinterpret_cast<uint4*>(out + dlo) = lo[u];
-        *reinterpret_cast<uint4*>(out + dhi) = hi[u];
+        out += ((int64_t)it.row * it.N + h) * p.H;
+        *reinterpret_cast<uint4*>(out + l.dlo) = lo;
+        *reinterpret_cast<uint4*>(out + l.dhi) = hi;
       }
     }
     if (LANES == 4 || LANES == 8) {  // the head sizes of the cache
-      if (p.cached && kind > 0)      // the whole warp takes part in the ranges' shuffles
-        prep_to_cache<LANES>(write ? i4_head(p.c, seq, place, h, 36 * p.H) : nullptr, (int)(place % kI4Page), kind == 2, p.H, dlo, dhi, lo[u], hi[u], sub);
+      if (p.cached && it.kind > 0)   // the whole warp takes part in the ranges' shuffles
+        prep_to_cache<LANES>(write ? i4_head(p.c, it.seq, it.place, h, 36 * p.H) : nullptr, (int)(it.place % kI4Page), it.kind == 2, p.H, l.dlo, l.dhi, lo, hi, l.sub);
     }
   }
+}
+
+// Few tokens: a warp per item, a head per thread, loads straight to registers
+template <int LANES>
+__global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int item = (int)(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+  if (item >= p.T * p.wpt) return;  // a warp as a whole
+  const PrepLane l = prep_lane<LANES>(p, lane);
+  const PrepItem it = prep_item<LANES>(p, item);
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  if (l.live && it.base + lane / LANES < it.N) {
+    const uint16_t* src = prep_source(p, it) + (it.base + lane / LANES) * p.H;
+    lo = *reinterpret_cast<const uint4*>(src + l.dlo);
+    hi = *reinterpret_cast<const uint4*>(src + l.dhi);
+  }
+  if (it.seq < 0) return;  // a row of no sequence
+  prep_heads<LANES, 1>(p, it, l, lane, [&](int, uint4& a, uint4& b) { a = lo; b = hi; },
+                       [&](float(&cs)[8], float(&sn)[8]) {
+                         prep_weights(p.ep + it.pos * p.ld_ep, 1, l.dlo, cs);
+                         prep_weights(p.ep + (p.max_pos + it.pos) * p.ld_ep, 1, l.dlo, sn);
+                       });
+}
+
+// Many tokens: resident warps walk the items, four heads per thread. The next item's pieces and angles come by cp.async while this one is
+// worked on, each lane's into places of its own (no barrier): with loads to registers 16 warps per SM had too little in flight (8191
+// tokens, 40 heads of 128: 51 us, 3.4 TB/s).
+constexpr int kPrepUnits = 4, kPrepWarps = 8;
+constexpr int kPrepStage = (2 * kPrepUnits + 4) * 512;  // bytes per warp: two pieces of each head, four of cosines and sines
+template <int LANES>
+__global__ void __launch_bounds__(kPrepWarps * 32, 2) head_prep_many_kernel(const PrepParams p) {
+  extern __shared__ __align__(16) unsigned char prep_smem[];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = p.stride, items = p.T * p.wpt;
+  unsigned char* mine = prep_smem + warp * 2 * kPrepStage + lane * 16;
+  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+  const PrepLane l = prep_lane<LANES>(p, lane);
+  auto copy = [&](int piece, int stage, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine_s + stage * kPrepStage + piece * 512), "l"(src) : "memory");
+  };
+  auto fetch = [&](const PrepItem& it, int stage) {
+    const uint16_t* src = prep_source(p, it);
+#pragma unroll
+    for (int u = 0; u < kPrepUnits; u++) {
+      const int h = it.base + lane / LANES + u * it.groups;
+      if (l.live && h < it.N) {
+        copy(2 * u, stage, src + h * p.H + l.dlo);
+        copy(2 * u + 1, stage, src + h * p.H + l.dhi);
+      }
+    }
+    if (l.turns && it.pos >= 0) {
+      const float *c = p.ep + it.pos * p.ld_ep + l.dlo, *s = c + p.max_pos * p.ld_ep;
+      copy(2 * kPrepUnits, stage, c);
+      copy(2 * kPrepUnits + 1, stage, c + 4);
+      copy(2 * kPrepUnits + 2, stage, s);
+      copy(2 * kPrepUnits + 3, stage, s + 4);
+    }
+  };
+  // items of one warp are taken in the order of the rows; the one after the next is looked up a round ahead
+  int i = blockIdx.x * kPrepWarps + warp;
+  if (i >= min(warps, items)) return;
+  PrepItem now = prep_item<LANES>(p, i), ahead = now;
+  fetch(now, 0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (i + warps < items) ahead = prep_item<LANES>(p, i + warps);
+  for (int stage = 0; i < items; i += warps, stage ^= 1) {
+    if (i + warps < items) fetch(ahead, stage ^ 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    PrepItem later = ahead;
+    if (i + 2 * warps < items) later = prep_item<LANES>(p, i + 2 * warps);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const unsigned char* at = mine + stage * kPrepStage;
+    auto piece = [&](int k) { return *reinterpret_cast<const uint4*>(at + k * 512); };
+    if (now.seq >= 0)
+      prep_heads<LANES, kPrepUnits>(p, now, l, lane,
+                                    [&](int u, uint4& a, uint4& b) {
+                                      a = piece(2 * u);
+                                      b = piece(2 * u + 1);
+                                      if (!l.live || now.base + lane / LANES + u * now.groups >= now.N) a = b = make_uint4(0, 0, 0, 0);
+                                    },
+                                    [&](float(&cs)[8], float(&sn)[8]) {
+#pragma unroll
+                                      for (int k = 0; k < 2; k++) {
+                                        const uint4 c = piece(2 * kPrepUnits + k), s = piece(2 * kPrepUnits + 2 + k);
+                                        const uint32_t cw[4] = {c.x, c.y, c.z, c.w}, sw[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                                        for (int j = 0; j < 4; j++) {
+                                          cs[4 * k + j] = __uint_as_float(cw[j]);
+                                          sn[4 * k + j] = __uint_as_float(sw[j]);
+                                        }
+                                      }
+                                    });
+    now = ahead;
+    ahead = later;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // A thread has one piece of 8 values of up to UNITS heads of a token: where the token is found once, and the loads go out together.
@@ -338,17 +451,30 @@ int i4_cache_of(const TpxInt4Cache* a, I4Cache* c) {
 
 template <int LANES>
 static int prep_launch(PrepParams& p, cudaStream_t st) {
-  // Four heads per thread once that still fills the GPU
   const int heads = p.Nq + p.Nkv + (p.cached ? p.Nkv : 0);
+  // Four heads per thread and resident warps once that gives every warp an item or more
   const bool many = (int64_t)p.T * heads * LANES >= (int64_t)sm_count() * 2048;
-  const int per_warp = 32 / LANES * (many ? 4 : 1), block = 256;
+  const int per_warp = 32 / LANES * (many ? kPrepUnits : 1);
   p.wq = (p.Nq + per_warp - 1) / per_warp;
   p.wkv = (p.Nkv + per_warp - 1) / per_warp;
   p.wpt = p.wq + (p.cached ? 2 : 1) * p.wkv;
-  const int64_t grid = ((int64_t)p.T * p.wpt + block / 32 - 1) / (block / 32);
-  TPX_REQUIRE(grid * (block / 32) < (1ll << 31), TPX_ERR_UNSUPPORTED, "head_prep: too many tokens in one call");
-  TPX_CUDA_OK(many ? launch_pdl(head_prep_kernel<LANES, 4>, dim3((unsigned)grid), dim3(block), 0, st, p)
-                   : launch_pdl(head_prep_kernel<LANES, 1>, dim3((unsigned)grid), dim3(block), 0, st, p));
+  TPX_REQUIRE((int64_t)p.T * p.wpt < (1ll << 30), TPX_ERR_UNSUPPORTED, "head_prep: too many tokens in one call");
+  if (!many) {
+    TPX_CUDA_OK(launch_pdl(head_prep_kernel<LANES>, dim3((p.T * p.wpt + 7) / 8), dim3(256), 0, st, p));
+    return TPX_OK;
+  }
+  // no common factor with the items of a token: every warp then meets all kinds, which take different times
+  p.stride = 2 * sm_count() * kPrepWarps;
+  while (std::gcd(p.stride, p.wpt) != 1) p.stride--;
+  constexpr int SMEM = kPrepWarps * 2 * kPrepStage;
+  static bool opted[16] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16 || !opted[dev]) {
+    TPX_CUDA_OK(cudaFuncSetAttribute(head_prep_many_kernel<LANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev >= 0 && dev < 16) opted[dev] = true;
+  }
+  TPX_CUDA_OK(launch_pdl(head_prep_many_kernel<LANES>, dim3(2 * sm_count()), dim3(kPrepWarps * 32), SMEM, st, p));
   return TPX_OK;
 }
 
@@ -369,7 +495,7 @@ extern "C" int tpx_head_prep(const TpxHeadPrep* a, void* stream) {
                    (uintptr_t)a->k_norm | (uintptr_t)a->ep;
   TPX_REQUIRE((bits & 15) == 0 && (a->ldq | a->ldk | a->ldv) % 8 == 0, TPX_ERR_ARG, "head_prep: tensors and their rows must be 16-byte aligned");
   PrepParams p = {a->q, a->k, a->v, a->q_norm, a->k_norm, a->ep, a->pos, a->cu_seqlens, a->q_out, a->k_out, {}, a->ldq, a->ldk, a->ldv, a->max_pos, a->ld_ep,
-                  (int)a->T, (int)a->Nq, (int)a->Nkv, (int)a->H, a->ep ? (int)a->rot : 0, 0, 0, 0, a->eps, a->norm_is_f32, 0};
+                  (int)a->T, (int)a->Nq, (int)a->Nkv, (int)a->H, a->ep ? (int)a->rot : 0, 0, 0, 0, 0, a->eps, 1.0f / (float)a->H, a->norm_is_f32, 0};
   if (a->cache) {
     const int rc = i4_cache_of(a->cache, &p.c);
     if (rc) return rc;
