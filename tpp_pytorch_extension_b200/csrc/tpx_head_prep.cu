@@ -130,28 +130,33 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
     for (int g = 0; g < H / kI4Group; g++) params[g] = param[g];
 }
 
-// Pairs of fp32 in one operation
-__device__ __forceinline__ float2 prep_fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{ .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Pairs of fp32 in one operation, kept in 64-bit registers
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 prep_pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
   return r;
 }
-__device__ __forceinline__ float2 prep_mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{ .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w; }"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ void prep_halves(f32x2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a)); }
+__device__ __forceinline__ f32x2 prep_fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ void prep_pairs(uint4 v, float2 (&x)[4]) {
+__device__ __forceinline__ f32x2 prep_mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void prep_pairs(uint4 v, f32x2 (&x)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int j = 0; j < 4; j++) x[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+  for (int j = 0; j < 4; j++) x[j] = prep_pair(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
 }
-__device__ __forceinline__ uint4 prep_pack(const float2 (&x)[4]) {
-  const float f[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+__device__ __forceinline__ uint4 prep_pack(const f32x2 (&x)[4]) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; j++) prep_halves(x[j], f[2 * j], f[2 * j + 1]);
   return prep_pack(f);
 }
 
@@ -159,13 +164,13 @@ __device__ __forceinline__ uint4 prep_pack(const float2 (&x)[4]) {
 struct PrepItem {
   int row, kind, N, groups, base;  // queries, keys, values; heads, distance of a thread's heads, the warp's first group
   int seq;                         // -1: a row of no sequence
-  int64_t place, pos;              // of the token in the cache; pos < 0: no rotation
+  int64_t place, pos;              // of the token in the cache, in the rotation table (outside: no rotation)
 };
+__device__ __forceinline__ bool prep_turns(const PrepParams& p, const PrepItem& it) { return (unsigned long long)it.pos < (unsigned long long)p.max_pos; }
 template <int LANES>
-__device__ __forceinline__ PrepItem prep_item(const PrepParams& p, int item) {
+__device__ __forceinline__ PrepItem prep_item(const PrepParams& p, int row, int in_row) {
   PrepItem it;
-  it.row = item / p.wpt;
-  const int in_row = item - it.row * p.wpt;
+  it.row = row;
   it.kind = in_row < p.wq ? 0 : in_row < p.wq + p.wkv ? 1 : 2;
   it.N = it.kind ? p.Nkv : p.Nq;
   it.groups = (it.kind ? p.wkv : p.wq) * (32 / LANES);
@@ -176,8 +181,7 @@ __device__ __forceinline__ PrepItem prep_item(const PrepParams& p, int item) {
     it.seq = i4_sequence(p.cu, p.c.B, it.row);
     if (it.seq >= 0) it.place = (int64_t)max(p.c.lengths[it.seq], 0) + (p.cu ? it.row - p.cu[it.seq] : 0);
   }
-  it.pos = it.kind == 2 || p.rot == 0 ? -1 : p.pos ? p.pos[it.row] : it.place;
-  if (it.pos >= p.max_pos) it.pos = -1;
+  it.pos = it.kind == 2 || p.rot == 0 ? -1 : p.pos ? p.pos[it.row] : it.place;  // looked at when the item is fetched, not here
   return it;
 }
 // A lane's pieces of a head: the first rot / 16 lanes hold rotary pairs, the others two pieces side by side
@@ -199,34 +203,37 @@ __device__ __forceinline__ const uint16_t* prep_source(const PrepParams& p, cons
   return it.kind == 0 ? p.q + it.row * p.ldq : it.kind == 1 ? p.k + it.row * p.ldk : p.v + it.row * p.ldv;
 }
 
-// The heads of an item: load(u, lo, hi) gives the thread's pieces of its head u, angles(cs, sn) its cosines and sines
-template <int LANES, int UNITS, class Load, class Angles>
-__device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& it, const PrepLane& l, int lane, Load load, Angles angles) {
-  const void* norm = it.kind == 0 ? p.q_norm : it.kind == 1 ? p.k_norm : nullptr;
-  const bool rotate = l.turns && it.pos >= 0, turned = __all_sync(0xffffffffu, rotate || !l.live);
+// The heads of an item: load(u, lo, hi) gives the thread's pieces of its head u, weights(wl, wh) those of the norm (or ones),
+// angles(cs, sn) its cosines and sines
+template <int LANES, int UNITS, class Load, class Weights, class Angles>
+__device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& it, const PrepLane& l, int lane, Load load, Weights weights, Angles angles) {
+  const bool norm = it.kind == 0 ? p.q_norm != nullptr : it.kind == 1 && p.k_norm != nullptr;
+  const bool rotate = l.turns && prep_turns(p, it), turned = __all_sync(0xffffffffu, rotate || !l.live);
   const int first = it.base + lane / LANES;
   // out_lo = x_lo (w_lo c) - x_hi (w_hi s), out_hi = x_hi (w_hi c) + x_lo (w_lo s)
-  float2 lc[4], hs[4], hc[4], ls[4];
+  f32x2 lc[4], hs[4], hc[4], ls[4];
   if (it.kind < 2) {
-    float wl[8], wh[8], cs[8], sn[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      wl[i] = wh[i] = cs[i] = 1.0f;
-      sn[i] = 0.0f;
-    }
-    if (norm && l.live) {
-      prep_weights(norm, p.norm_f32, l.dlo, wl);
-      prep_weights(norm, p.norm_f32, l.dhi, wh);
-    }
-    if (rotate) angles(cs, sn);
+    f32x2 wl[4], wh[4];
+    weights(wl, wh);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      lc[i] = make_float2(wl[2 * i] * cs[2 * i], wl[2 * i + 1] * cs[2 * i + 1]);
-      hs[i] = make_float2(-wh[2 * i] * sn[2 * i], -wh[2 * i + 1] * sn[2 * i + 1]);
-      hc[i] = make_float2(wh[2 * i] * cs[2 * i], wh[2 * i + 1] * cs[2 * i + 1]);
-      ls[i] = make_float2(wl[2 * i] * sn[2 * i], wl[2 * i + 1] * sn[2 * i + 1]);
+      lc[i] = wl[i];
+      hc[i] = wh[i];
+      hs[i] = ls[i] = 0;
+    }
+    if (rotate) {
+      f32x2 cs[4], sn[4];
+      angles(cs, sn);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        lc[i] = prep_mul2(wl[i], cs[i]);
+        hc[i] = prep_mul2(wh[i], cs[i]);
+        ls[i] = prep_mul2(wl[i], sn[i]);
+        hs[i] = prep_mul2(wh[i], sn[i]) ^ 0x8000000080000000ull;
+      }
     }
   }
+  uint16_t* const out0 = it.kind == 0 ? p.q_out : p.k_out;
 #pragma unroll
   for (int u = 0; u < UNITS; u++) {
     if (u * it.groups >= it.N) break;
@@ -235,18 +242,20 @@ __device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& 
     uint4 lo, hi;
     load(u, lo, hi);
     if (it.kind < 2) {
-      float2 a[4], b[4];
+      f32x2 a[4], b[4];
       prep_pairs(lo, a);
       prep_pairs(hi, b);
       if (norm) {
-        float2 s2 = make_float2(0.0f, 0.0f);
+        f32x2 s2 = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) s2 = prep_fma2(b[i], b[i], prep_fma2(a[i], a[i], s2));
-        float ss = s2.x + s2.y;
+        float s0, s1;
+        prep_halves(s2, s0, s1);
+        float ss = s0 + s1;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = rsqrtf(fmaf(ss, p.inv_h, p.eps));
-        const float2 inv2 = make_float2(inv, inv);
+        const f32x2 inv2 = prep_pair(inv, inv);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           a[i] = prep_mul2(a[i], inv2);
@@ -254,7 +263,7 @@ __device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& 
         }
       }
       if (norm || p.rot) {
-        float2 x[4], y[4];
+        f32x2 x[4], y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           x[i] = prep_mul2(a[i], lc[i]);
@@ -270,9 +279,8 @@ __device__ __forceinline__ void prep_heads(const PrepParams& p, const PrepItem& 
         lo = prep_pack(x);
         hi = prep_pack(y);
       }
-      uint16_t* out = it.kind == 0 ? p.q_out : p.k_out;
-      if (write && out) {
-        out += ((int64_t)it.row * it.N + h) * p.H;
+      if (write && out0) {
+        uint16_t* out = out0 + ((int64_t)it.row * it.N + h) * p.H;
         *reinterpret_cast<uint4*>(out + l.dlo) = lo;
         *reinterpret_cast<uint4*>(out + l.dhi) = hi;
       }
@@ -292,7 +300,7 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
   const int item = (int)(((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
   if (item >= p.T * p.wpt) return;  // a warp as a whole
   const PrepLane l = prep_lane<LANES>(p, lane);
-  const PrepItem it = prep_item<LANES>(p, item);
+  const PrepItem it = prep_item<LANES>(p, item / p.wpt, item % p.wpt);
   uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
   if (l.live && it.base + lane / LANES < it.N) {
     const uint16_t* src = prep_source(p, it) + (it.base + lane / LANES) * p.H;
@@ -300,14 +308,36 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
     hi = *reinterpret_cast<const uint4*>(src + l.dhi);
   }
   if (it.seq < 0) return;  // a row of no sequence
-  prep_heads<LANES, 1>(p, it, l, lane, [&](int, uint4& a, uint4& b) { a = lo; b = hi; },
-                       [&](float(&cs)[8], float(&sn)[8]) {
-                         prep_weights(p.ep + it.pos * p.ld_ep, 1, l.dlo, cs);
-                         prep_weights(p.ep + (p.max_pos + it.pos) * p.ld_ep, 1, l.dlo, sn);
-                       });
+  const void* norm = it.kind == 0 ? p.q_norm : p.k_norm;
+  auto pairs = [](const float(&f)[8], f32x2(&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = prep_pair(f[2 * i], f[2 * i + 1]);
+  };
+  prep_heads<LANES, 1>(
+      p, it, l, lane,
+      [&](int, uint4& a, uint4& b) {
+        a = lo;
+        b = hi;
+      },
+      [&](f32x2(&wl)[4], f32x2(&wh)[4]) {
+        float f[8] = {1, 1, 1, 1, 1, 1, 1, 1}, h[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+        if (norm && l.live) {
+          prep_weights(norm, p.norm_f32, l.dlo, f);
+          prep_weights(norm, p.norm_f32, l.dhi, h);
+        }
+        pairs(f, wl);
+        pairs(h, wh);
+      },
+      [&](f32x2(&cs)[4], f32x2(&sn)[4]) {
+        float f[8];
+        prep_weights(p.ep + it.pos * p.ld_ep, 1, l.dlo, f);
+        pairs(f, cs);
+        prep_weights(p.ep + (p.max_pos + it.pos) * p.ld_ep, 1, l.dlo, f);
+        pairs(f, sn);
+      });
 }
 
-// Many tokens: resident warps walk the items, four heads per thread. The next item's pieces and angles come by cp.async while this one is
+// Many tokens: resident warps walk the tokens, four heads per thread. The next token's pieces and angles come by cp.async while this one is
 // worked on, each lane's into places of its own (no barrier): with loads to registers 16 warps per SM had too little in flight (8191
 // tokens, 40 heads of 128: 51 us, 3.4 TB/s).
 constexpr int kPrepUnits = 4, kPrepWarps = 8;
@@ -315,67 +345,93 @@ constexpr int kPrepStage = (2 * kPrepUnits + 4) * 512;  // bytes per warp: two p
 template <int LANES>
 __global__ void __launch_bounds__(kPrepWarps * 32, 2) head_prep_many_kernel(const PrepParams p) {
   extern __shared__ __align__(16) unsigned char prep_smem[];
+  __shared__ __align__(16) float norms[2][LANES * 16];  // weights of queries and of keys, or ones
   pdl_trigger();
   pdl_wait();
+  for (int i = threadIdx.x; i < 2 * LANES * 16; i += kPrepWarps * 32) {
+    const void* w = i < LANES * 16 ? p.q_norm : p.k_norm;
+    const int d = i % (LANES * 16);
+    norms[i / (LANES * 16)][d] = !w || d >= p.H ? 1.0f : p.norm_f32 ? ((const float*)w)[d] : bf16_bits_to_f32(((const uint16_t*)w)[d]);
+  }
+  __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = p.stride, items = p.T * p.wpt;
+  int i = blockIdx.x * kPrepWarps + warp;
+  if (i >= min(warps, items)) return;
+  const PrepLane l = prep_lane<LANES>(p, lane);
   unsigned char* mine = prep_smem + warp * 2 * kPrepStage + lane * 16;
   const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
-  const PrepLane l = prep_lane<LANES>(p, lane);
-  auto copy = [&](int piece, int stage, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine_s + stage * kPrepStage + piece * 512), "l"(src) : "memory");
+  // what is not there (no such head, a lane without values, a token without angles) is filled with zeros
+  auto copy = [&](int piece, int stage, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine_s + stage * kPrepStage + piece * 512), "l"(src), "r"(valid ? 16 : 0) : "memory");
   };
   auto fetch = [&](const PrepItem& it, int stage) {
     const uint16_t* src = prep_source(p, it);
+    const int h0 = it.base + lane / LANES;
 #pragma unroll
     for (int u = 0; u < kPrepUnits; u++) {
-      const int h = it.base + lane / LANES + u * it.groups;
-      if (l.live && h < it.N) {
-        copy(2 * u, stage, src + h * p.H + l.dlo);
-        copy(2 * u + 1, stage, src + h * p.H + l.dhi);
-      }
+      const bool valid = l.live && h0 + u * it.groups < it.N;
+      const uint16_t* head = src + (valid ? (h0 + u * it.groups) * p.H : 0);
+      copy(2 * u, stage, head + (valid ? l.dlo : 0), valid);
+      copy(2 * u + 1, stage, head + (valid ? l.dhi : 0), valid);
     }
-    if (l.turns && it.pos >= 0) {
-      const float *c = p.ep + it.pos * p.ld_ep + l.dlo, *s = c + p.max_pos * p.ld_ep;
-      copy(2 * kPrepUnits, stage, c);
-      copy(2 * kPrepUnits + 1, stage, c + 4);
-      copy(2 * kPrepUnits + 2, stage, s);
-      copy(2 * kPrepUnits + 3, stage, s + 4);
+    if (p.rot && it.kind < 2) {
+      const bool valid = l.turns && prep_turns(p, it);
+      const float *c = p.ep + (valid ? it.pos * p.ld_ep + l.dlo : 0), *s = c + (valid ? p.max_pos * p.ld_ep : 0);
+      copy(2 * kPrepUnits, stage, c, valid);
+      copy(2 * kPrepUnits + 1, stage, c + (valid ? 4 : 0), valid);
+      copy(2 * kPrepUnits + 2, stage, s, valid);
+      copy(2 * kPrepUnits + 3, stage, s + (valid ? 4 : 0), valid);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // items of one warp are taken in the order of the rows; the one after the next is looked up a round ahead
-  int i = blockIdx.x * kPrepWarps + warp;
-  if (i >= min(warps, items)) return;
-  PrepItem now = prep_item<LANES>(p, i), ahead = now;
+  int row = i / p.wpt, in_row = i % p.wpt;
+  const int rows_on = warps / p.wpt, in_row_on = warps % p.wpt;
+  auto onward = [&]() {
+    row += rows_on;
+    in_row += in_row_on;
+    if (in_row >= p.wpt) {
+      in_row -= p.wpt;
+      row++;
+    }
+  };
+  PrepItem now = prep_item<LANES>(p, row, in_row), ahead = now;
   fetch(now, 0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  if (i + warps < items) ahead = prep_item<LANES>(p, i + warps);
+  onward();
+  if (i + warps < items) ahead = prep_item<LANES>(p, row, in_row);
   for (int stage = 0; i < items; i += warps, stage ^= 1) {
     if (i + warps < items) fetch(ahead, stage ^ 1);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    else asm volatile("cp.async.commit_group;" ::: "memory");
     PrepItem later = ahead;
-    if (i + 2 * warps < items) later = prep_item<LANES>(p, i + 2 * warps);
+    onward();
+    if (i + 2 * warps < items) later = prep_item<LANES>(p, row, in_row);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     const unsigned char* at = mine + stage * kPrepStage;
-    auto piece = [&](int k) { return *reinterpret_cast<const uint4*>(at + k * 512); };
+    auto four = [](const void* from, f32x2& a, f32x2& b) {  // of 16 bytes
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(from);
+      a = v.x;
+      b = v.y;
+    };
     if (now.seq >= 0)
-      prep_heads<LANES, kPrepUnits>(p, now, l, lane,
-                                    [&](int u, uint4& a, uint4& b) {
-                                      a = piece(2 * u);
-                                      b = piece(2 * u + 1);
-                                      if (!l.live || now.base + lane / LANES + u * now.groups >= now.N) a = b = make_uint4(0, 0, 0, 0);
-                                    },
-                                    [&](float(&cs)[8], float(&sn)[8]) {
-#pragma unroll
-                                      for (int k = 0; k < 2; k++) {
-                                        const uint4 c = piece(2 * kPrepUnits + k), s = piece(2 * kPrepUnits + 2 + k);
-                                        const uint32_t cw[4] = {c.x, c.y, c.z, c.w}, sw[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                                        for (int j = 0; j < 4; j++) {
-                                          cs[4 * k + j] = __uint_as_float(cw[j]);
-                                          sn[4 * k + j] = __uint_as_float(sw[j]);
-                                        }
-                                      }
-                                    });
+      prep_heads<LANES, kPrepUnits>(
+          p, now, l, lane,
+          [&](int u, uint4& a, uint4& b) {
+            a = *reinterpret_cast<const uint4*>(at + 2 * u * 512);
+            b = *reinterpret_cast<const uint4*>(at + (2 * u + 1) * 512);
+          },
+          [&](f32x2(&wl)[4], f32x2(&wh)[4]) {
+            const float* w = norms[now.kind];
+            four(w + l.dlo, wl[0], wl[1]);
+            four(w + l.dlo + 4, wl[2], wl[3]);
+            four(w + l.dhi, wh[0], wh[1]);
+            four(w + l.dhi + 4, wh[2], wh[3]);
+          },
+          [&](f32x2(&cs)[4], f32x2(&sn)[4]) {
+            four(at + 2 * kPrepUnits * 512, cs[0], cs[1]);
+            four(at + (2 * kPrepUnits + 1) * 512, cs[2], cs[3]);
+            four(at + (2 * kPrepUnits + 2) * 512, sn[0], sn[1]);
+            four(at + (2 * kPrepUnits + 3) * 512, sn[2], sn[3]);
+          });
     now = ahead;
     ahead = later;
   }
@@ -453,7 +509,7 @@ template <int LANES>
 static int prep_launch(PrepParams& p, cudaStream_t st) {
   const int heads = p.Nq + p.Nkv + (p.cached ? p.Nkv : 0);
   // Four heads per thread and resident warps once that gives every warp an item or more
-  const bool many = (int64_t)p.T * heads * LANES >= (int64_t)sm_count() * 2048;
+  const bool many = (int64_t)p.T * heads * LANES >= (int64_t)sm_count() * 2048 && heads <= 2048;
   const int per_warp = 32 / LANES * (many ? kPrepUnits : 1);
   p.wq = (p.Nq + per_warp - 1) / per_warp;
   p.wkv = (p.Nkv + per_warp - 1) / per_warp;
