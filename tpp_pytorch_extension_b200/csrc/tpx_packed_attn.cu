@@ -97,6 +97,56 @@ __device__ __forceinline__ float pk_ex2(float x) {  // 2^-inf = 0
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float pk_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// pairs of fp32 in 64-bit registers
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pk_pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void pk_halves(f32x2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a)); }
+__device__ __forceinline__ f32x2 pk_fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 pk_add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 pk_mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of a pair without the special-function unit: x = n + f with n the nearest whole number (1.5 * 2^23 brings it to the low bits), a polynomial of degree 4
+// in f, -1/2 <= f <= 1/2, with the smallest relative error (2.6e-6, fitted for this kernel), and n added to its exponent. x below -126 gives
+// 2^-126 or so in the place of less.
+__device__ __forceinline__ f32x2 pk_exp2_pair(f32x2 x) {
+  float a, b;
+  pk_halves(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
+  x = pk_pair(a, b);
+  const f32x2 big = pk_pair(12582912.0f, 12582912.0f), t = pk_add2(x, big), n = pk_add2(t, pk_pair(-12582912.0f, -12582912.0f));
+  const f32x2 f = pk_fma2(n, pk_pair(-1.0f, -1.0f), x);
+  f32x2 y = pk_fma2(pk_pair(0.009570101276040077f, 0.009570101276040077f), f, pk_pair(0.05591785907745361f, 0.05591785907745361f));
+  y = pk_fma2(y, f, pk_pair(0.240247443318367f, 0.240247443318367f));
+  y = pk_fma2(y, f, pk_pair(0.6931217908859253f, 0.6931217908859253f));
+  y = pk_fma2(y, f, pk_pair(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb;
+  pk_halves(t, ta, tb);
+  pk_halves(y, a, b);
+  a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
+  b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
+  return pk_fma2(f, 0, pk_pair(a, b));  // a NaN, which the addition to the exponent has undone
+}
 __device__ __forceinline__ uint32_t pk_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -117,6 +167,8 @@ struct PkUnit {
   int tok0, n, t0, head;  // first row of the sequence, its tokens, the unit's first token, key head
   int tiles[2];           // key tiles that A and B walk; 0: no such tile
 };
+// The units of a block: rounds over all blocks, every other one backwards, since units get shorter along a sequence (causal)
+__device__ __forceinline__ int pk_nth(int round) { return round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); }
 // Unit u of the call: sequences in order, the last tokens (with the most keys) of a sequence first, heads of the same tokens side by side
 __device__ __forceinline__ PkUnit pk_unit(const PkParams& p, const int* pre, int buckets, int stride, int u) {
   PkUnit w;
@@ -150,7 +202,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                    const PkParams p) {
   using C = PkCfg<H>;
   extern __shared__ unsigned char pk_smem_raw[];
-  __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free[2], kv_full[C::SLOTS], kv_empty[C::SLOTS];
+  __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_free[2], kv_full[C::SLOTS], kv_empty[C::SLOTS];
   __shared__ uint32_t tmem_holder;
   __shared__ int dirty;  // some value in a tile's margin is not finite
   __shared__ int pre[kPkBuckets + 1], warp_sum[kPkThreads / 32];
@@ -165,6 +217,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       tc_mbar_init(tc_smem_u32(&q_full[x]), 1);
       tc_mbar_init(tc_smem_u32(&q_empty[x]), 1);
       tc_mbar_init(tc_smem_u32(&s_full[x]), 1);
+      tc_mbar_init(tc_smem_u32(&p_half[x]), 128);
       tc_mbar_init(tc_smem_u32(&p_full[x]), 128);
       tc_mbar_init(tc_smem_u32(&o_full[x]), 1);
       tc_mbar_init(tc_smem_u32(&o_free[x]), 128);
@@ -225,7 +278,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const uint32_t q_bytes = (uint32_t)(C::HALVES * p.TPT * p.R * 128);
       int seen[2] = {0, 0}, c = 0;  // units of each tile, ring slots so far
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      for (int round = 0; ok && round * (int)gridDim.x < units; round++) {
+        const int u = pk_nth(round);
+        if (u >= units) continue;
         const PkUnit w = pk_unit(p, pre, buckets, stride, u);
         const int n = max(w.tiles[0], w.tiles[1]);
         auto load_q = [&](int x) {
@@ -288,7 +343,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         tc_commit(tc_smem_u32(&s_full[x]));
       };
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      for (int round = 0; ok && round * (int)gridDim.x < units; round++) {
+        const int u = pk_nth(round);
+        if (u >= units) continue;
         const PkUnit w = pk_unit(p, pre, buckets, stride, u);
         const int n = max(w.tiles[0], w.tiles[1]);
         if (!wait(&kv_full[c % C::SLOTS], c / C::SLOTS)) break;  // keys of tile 0
@@ -303,13 +360,16 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           for (int x = 0; ok && x < 2; x++) {
             if (j >= w.tiles[x]) continue;
             if (j == 0 && seen[x] && !wait(&o_free[x], seen[x] - 1)) break;
-            if (!wait(&p_full[x], steps[x])) break;
-            steps[x]++;
-            tc_fence_after();
+            for (int half = 0; ok && half < 2; half++) {  // weights of the first, of the last 64 keys
+              if (!wait(half ? &p_full[x] : &p_half[x], steps[x])) break;
+              tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)  // 16 keys: 8 columns of packed weights, two 8-key groups of values
-              pk_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + kk * 8, pk_desc_mn(kv_s + vs * C::TILE_BYTES + kk * 2048, C::HALF_BYTES), idesc_o,
-                        j > 0 || kk > 0 ? 1u : 0u);
+              for (int kk = half * 4; kk < half * 4 + 4; kk++)  // 16 keys: 8 columns of packed weights, two 8-key groups of values
+                pk_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + kk * 8, pk_desc_mn(kv_s + vs * C::TILE_BYTES + kk * 2048, C::HALF_BYTES), idesc_o,
+                          j > 0 || kk > 0 ? 1u : 0u);
+            }
+            if (!ok) break;
+            steps[x]++;
             if (j + 1 < w.tiles[x]) {
               scores(x, ks);
             } else {
@@ -346,7 +406,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       }
       return ok;
     };
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+    for (int round = 0; ok && round * (int)gridDim.x < units; round++) {
+      const int u = pk_nth(round);
+      if (u >= units) continue;
       const PkUnit w = pk_unit(p, pre, buckets, stride, u);
       const int n_all = max(w.tiles[0], w.tiles[1]), n = w.tiles[x];
       const int c0 = c;  // the unit's first ring slot; values of tile j are in slot c0 + 1 + 2 j
@@ -357,6 +419,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const int klim = p.causal ? min(t + 1, w.n) : w.n;               // keys [0, klim) are seen (dead rows: anything)
       const int whole = (p.causal ? w.t0 + 1 : w.n) / 128;              // key tiles that every row of the unit sees in full
       float m_ref = -INFINITY, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      f32x2 l2[2] = {0, 0};  // two more pairs of partial sums
       for (int j = 0; j < n; j++) {
         if (!wait(&s_full[x], steps)) break;
         steps++;
@@ -381,8 +444,10 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < 128; i++) top4[i & 3] = fmaxf(top4[i & 3], s[i]);
-        float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++) top4[k] = pk_max3(top4[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        float top = pk_max3(pk_max3(top4[0], top4[1], top4[2]), pk_max3(top4[3], s[124], s[125]), fmaxf(s[126], s[127]));
         // The multiply-add below takes the rounded reference off an unrounded score, which is nothing for ordinary scores; large ones are
         // rounded first, so that the largest weight is what it should be
         if (__any_sync(0xffffffffu, !(fabsf(top) * unit < 4096.0f)) && unit != 1.0f) {
@@ -398,6 +463,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           m_ref = m_new;
 #pragma unroll
           for (int i = 0; i < 4; i++) l[i] *= alpha;
+          l2[0] = pk_mul2(l2[0], pk_pair(alpha, alpha));
+          l2[1] = pk_mul2(l2[1], pk_pair(alpha, alpha));
           if (j > 0) {
 #pragma unroll
             for (int i = 0; i < H / 32; i++) {
@@ -409,18 +476,6 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               pk_st32(o_t + i * 32, o);
             }
           }
-        }
-        const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          uint32_t pw[32];
-#pragma unroll
-          for (int k = 0; k < 32; k++) {
-            const float a = pk_ex2(fmaf(s[64 * i + 2 * k], unit, -ref)), b = pk_ex2(fmaf(s[64 * i + 2 * k + 1], unit, -ref));
-            l[k & 3] += a + b;
-            pw[k] = pk_pack(a, b);
-          }
-          pk_st32(s_t + i * 32, pw);
         }
         if (margin) {
           const int vc = c0 + 1 + 2 * j;
@@ -449,6 +504,45 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           }
         }
+        const float ref = m_ref == -INFINITY ? 0.0f : m_ref;
+        const f32x2 unit2 = pk_pair(unit, unit), ref2 = pk_pair(-ref, -ref);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          uint32_t pw[32];
+          if (margin) {
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+              const float a = pk_ex2(fmaf(s[64 * i + 2 * k], unit, -ref)), b = pk_ex2(fmaf(s[64 * i + 2 * k + 1], unit, -ref));
+              l[k & 3] += a + b;
+              pw[k] = pk_pack(a, b);
+            }
+          } else {
+            // the special-function unit is as busy as the tensor core (16 of 2^x, 8192 products per clock): every third pair goes to the multiply-adds
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+              f32x2 e = pk_fma2(pk_pair(s[64 * i + 2 * k], s[64 * i + 2 * k + 1]), unit2, ref2);
+              float a, b;
+              if (k % 3 == 2) {
+                e = pk_exp2_pair(e);
+                pk_halves(e, a, b);
+              } else {
+                pk_halves(e, a, b);
+                a = pk_ex2(a);
+                b = pk_ex2(b);
+                e = pk_pair(a, b);
+              }
+              l2[k & 1] = pk_add2(l2[k & 1], e);
+              pw[k] = pk_pack(a, b);
+            }
+          }
+          pk_st32(s_t + i * 32, pw);
+          if (i == 0) {
+            __syncwarp();
+            pk_st_wait();
+            tc_fence_before();
+            tc_mbar_arrive(tc_smem_u32(&p_half[x]));
+          }
+        }
         __syncwarp();
         pk_st_wait();
         tc_fence_before();
@@ -457,7 +551,10 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (!wait(&o_full[x], seen)) break;
       seen++;
       tc_fence_after();
-      const float inv = 1.0f / ((l[0] + l[1]) + (l[2] + l[3]));
+      float more[4];
+      pk_halves(l2[0], more[0], more[1]);
+      pk_halves(l2[1], more[2], more[3]);
+      const float inv = 1.0f / (((l[0] + l[1]) + (l[2] + l[3])) + ((more[0] + more[1]) + (more[2] + more[3])));
       const bool mend = *reinterpret_cast<volatile int*>(&dirty) != 0;
       uint16_t* dst = p.out + ((int64_t)(w.tok0 + (live ? t : 0)) * p.Nq + w.head * p.R + member) * H;
 #pragma unroll
