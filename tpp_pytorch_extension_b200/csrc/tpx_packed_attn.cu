@@ -157,40 +157,54 @@ __device__ __forceinline__ void pk_sequence(const PkParams& p, int b, int& first
   first = min(max(p.cu[b], 0), p.T);
   n = max(min(max(p.cu[b + 1], 0), p.T) - first, 0);
 }
+// Units of a sequence. One that fills a single tile has its key heads in pairs, a tile each with keys of its own: units of one tile leave half of a
+// block idle and every step of it waiting for the one before (24 prompts of up to 300 tokens, 32 heads of 64: 42.7 us)
 __device__ __forceinline__ int pk_units(const PkParams& p, int b) {
   int first, n;
   pk_sequence(p, b, first, n);
-  return (n + 2 * p.TPT - 1) / (2 * p.TPT);
+  return n <= p.TPT ? (n > 0 ? (p.Nkv + 1) / 2 : 0) : (n + 2 * p.TPT - 1) / (2 * p.TPT) * p.Nkv;
 }
 
 struct PkUnit {
-  int tok0, n, t0, head;  // first row of the sequence, its tokens, the unit's first token, key head
-  int tiles[2];           // key tiles that A and B walk; 0: no such tile
+  int tok0, n;            // first row of the sequence, its tokens
+  int t0[2], head[2];     // first token and key head of tile A and B
+  int tiles[2];           // key tiles that they walk; 0: no such tile
+  bool split;             // the tiles have keys of their own, one tile each: ring slots are K A, K B, V A, V B (K, V without a tile B)
 };
 // The units of a block: rounds over all blocks, every other one backwards, since units get shorter along a sequence (causal)
 __device__ __forceinline__ int pk_nth(int round) { return round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); }
 // Unit u of the call: sequences in order, the last tokens (with the most keys) of a sequence first, heads of the same tokens side by side
 __device__ __forceinline__ PkUnit pk_unit(const PkParams& p, const int* pre, int buckets, int stride, int u) {
   PkUnit w;
-  const int su = u / p.Nkv;
-  w.head = u % p.Nkv;
-  int lo = 0, hi = buckets;  // pre[lo] <= su < pre[hi]
+  int lo = 0, hi = buckets;  // pre[lo] <= u < pre[hi]
   while (hi - lo > 1) {
     const int m = (lo + hi) >> 1;
-    if (pre[m] <= su) lo = m;
+    if (pre[m] <= u) lo = m;
     else hi = m;
   }
   int at = pre[lo], b = lo * stride, units = 0;
   for (; b < p.B; b++) {
     units = pk_units(p, b);
-    if (su < at + units) break;
+    if (u < at + units) break;
     at += units;
   }
   pk_sequence(p, min(b, p.B - 1), w.tok0, w.n);
-  w.t0 = (units - 1 - (su - at)) * 2 * p.TPT;
+  const int k = u - at;
+  w.split = w.n <= p.TPT;
+  if (w.split) {
+    w.t0[0] = w.t0[1] = 0;
+    w.head[0] = 2 * k;
+    w.head[1] = 2 * k + 1;
+    w.tiles[0] = 1;
+    w.tiles[1] = 2 * k + 1 < p.Nkv;
+    return w;
+  }
+  const int pair = units / p.Nkv - 1 - k / p.Nkv;
+  w.head[0] = w.head[1] = k % p.Nkv;
 #pragma unroll
   for (int x = 0; x < 2; x++) {
-    const int first = w.t0 + x * p.TPT, last = min(first + p.TPT, w.n) - 1;
+    const int first = (2 * pair + x) * p.TPT, last = min(first + p.TPT, w.n) - 1;
+    w.t0[x] = first;
     w.tiles[x] = first >= w.n ? 0 : ((p.causal ? last + 1 : w.n) + 127) / 128;
   }
   return w;
@@ -267,7 +281,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_holder;
-  const int units = total * p.Nkv;
+  const int units = total;
 
   // 384 x 168 registers at launch = 256 x 216 + 128 x 72
   if (warp < 4) {
@@ -291,9 +305,9 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           tc_mbar_expect_tx(bar, q_bytes);
 #pragma unroll
           for (int h = 0; h < C::HALVES; h++)  // 64 values x R members x 1 key head x TPT tokens
-            pk_tma_4d(q_s + x * C::TILE_BYTES + h * C::HALF_BYTES, &tmQ, h * 64, 0, w.head, w.tok0 + w.t0 + x * p.TPT, bar);
+            pk_tma_4d(q_s + x * C::TILE_BYTES + h * C::HALF_BYTES, &tmQ, h * 64, 0, w.head[x], w.tok0 + w.t0[x], bar);
         };
-        auto load_kv = [&](const CUtensorMap* map, int j) {
+        auto load_kv = [&](const CUtensorMap* map, int j, int x) {
           const int s = c % C::SLOTS;
           if (c >= C::SLOTS && !tc_wait(tc_smem_u32(&kv_empty[s]), (uint32_t)((c / C::SLOTS - 1) & 1))) { ok = false; return; }
           c++;
@@ -301,14 +315,20 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           tc_mbar_expect_tx(bar, C::TILE_BYTES);
 #pragma unroll
           for (int h = 0; h < C::HALVES; h++)
-            pk_tma_3d(kv_s + s * C::TILE_BYTES + h * C::HALF_BYTES, map, h * 64, w.head, w.tok0 + j * 128, bar);
+            pk_tma_3d(kv_s + s * C::TILE_BYTES + h * C::HALF_BYTES, map, h * 64, w.head[x], w.tok0 + j * 128, bar);
         };
         load_q(0);
-        if (ok) load_kv(&tmK, 0);
+        if (ok) load_kv(&tmK, 0, 0);
         if (ok) load_q(1);
+        if (w.split) {
+          if (ok && w.tiles[1]) load_kv(&tmK, 0, 1);
+          if (ok) load_kv(&tmV, 0, 0);
+          if (ok && w.tiles[1]) load_kv(&tmV, 0, 1);
+          continue;
+        }
         for (int j = 0; ok && j < n; j++) {
-          load_kv(&tmV, j);
-          if (ok && j + 1 < n) load_kv(&tmK, j + 1);
+          load_kv(&tmV, j, 0);
+          if (ok && j + 1 < n) load_kv(&tmK, j + 1, 0);
         }
       }
       if (!ok) {  // copies in flight land before this block gives its shared memory back
@@ -348,17 +368,34 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (u >= units) continue;
         const PkUnit w = pk_unit(p, pre, buckets, stride, u);
         const int n = max(w.tiles[0], w.tiles[1]);
-        if (!wait(&kv_full[c % C::SLOTS], c / C::SLOTS)) break;  // keys of tile 0
-        for (int x = 0; x < 2; x++)
-          if (w.tiles[x] && wait(&q_full[x], seen[x])) scores(x, c % C::SLOTS);
-        tc_commit(tc_smem_u32(&kv_empty[c % C::SLOTS]));
-        c++;
+        for (int x = 0; ok && x < 2; x++) {  // scores of the first keys
+          if (w.tiles[x] == 0) continue;
+          if ((x == 0 || w.split) && !wait(&kv_full[c % C::SLOTS], c / C::SLOTS)) break;
+          if (!wait(&q_full[x], seen[x])) break;
+          scores(x, c % C::SLOTS);
+          if (w.split) {
+            tc_commit(tc_smem_u32(&kv_empty[c % C::SLOTS]));
+            c++;
+          }
+        }
+        if (!ok) break;
+        if (!w.split) {
+          tc_commit(tc_smem_u32(&kv_empty[c % C::SLOTS]));
+          c++;
+        }
         for (int j = 0; ok && j < n; j++) {
-          const int vs = c % C::SLOTS, ks = (c + 1) % C::SLOTS;
+          int vs = c % C::SLOTS;
+          const int ks = (c + 1) % C::SLOTS;
           if (!wait(&kv_full[vs], c / C::SLOTS)) break;
           if (j + 1 < n && !wait(&kv_full[ks], (c + 1) / C::SLOTS)) break;
           for (int x = 0; ok && x < 2; x++) {
             if (j >= w.tiles[x]) continue;
+            if (w.split && x == 1) {  // values of its own
+              tc_commit(tc_smem_u32(&kv_empty[vs]));
+              c++;
+              vs = c % C::SLOTS;
+              if (!wait(&kv_full[vs], c / C::SLOTS)) break;
+            }
             if (j == 0 && seen[x] && !wait(&o_free[x], seen[x] - 1)) break;
             for (int half = 0; ok && half < 2; half++) {  // weights of the first, of the last 64 keys
               if (!wait(half ? &p_full[x] : &p_half[x], steps[x])) break;
@@ -412,12 +449,12 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const PkUnit w = pk_unit(p, pre, buckets, stride, u);
       const int n_all = max(w.tiles[0], w.tiles[1]), n = w.tiles[x];
       const int c0 = c;  // the unit's first ring slot; values of tile j are in slot c0 + 1 + 2 j
-      c += 2 * n_all;
+      c += w.split ? 2 * (w.tiles[0] + w.tiles[1]) : 2 * n_all;
       if (n == 0) continue;
-      const int t = w.t0 + x * p.TPT + tok;
+      const int t = w.t0[x] + tok;
       const bool live = tok < p.TPT && t < w.n;
       const int klim = p.causal ? min(t + 1, w.n) : w.n;               // keys [0, klim) are seen (dead rows: anything)
-      const int whole = (p.causal ? w.t0 + 1 : w.n) / 128;              // key tiles that every row of the unit sees in full
+      const int whole = (p.causal ? w.t0[0] + 1 : w.n) / 128;              // key tiles that every row of the unit sees in full
       float m_ref = -INFINITY, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       f32x2 l2[2] = {0, 0};  // two more pairs of partial sums
       for (int j = 0; j < n; j++) {
@@ -478,7 +515,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           }
         }
         if (margin) {
-          const int vc = c0 + 1 + 2 * j;
+          const int vc = w.split ? c0 + w.tiles[0] + w.tiles[1] + x : c0 + 1 + 2 * j;
           if (!wait(&kv_full[vc % C::SLOTS], vc / C::SLOTS)) break;
           const uint32_t base = kv_s + (vc % C::SLOTS) * C::TILE_BYTES + wg_tid * 16;
           const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
@@ -556,7 +593,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       pk_halves(l2[1], more[2], more[3]);
       const float inv = 1.0f / (((l[0] + l[1]) + (l[2] + l[3])) + ((more[0] + more[1]) + (more[2] + more[3])));
       const bool mend = *reinterpret_cast<volatile int*>(&dirty) != 0;
-      uint16_t* dst = p.out + ((int64_t)(w.tok0 + (live ? t : 0)) * p.Nq + w.head * p.R + member) * H;
+      uint16_t* dst = p.out + ((int64_t)(w.tok0 + (live ? t : 0)) * p.Nq + w.head[x] * p.R + member) * H;
 #pragma unroll
       for (int i = 0; i < H / 32; i++) {
         uint32_t o[32];
@@ -564,7 +601,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         pk_ld_wait();
         if (live && mend) {
           for (int key = whole * 128; key < klim; key++) {
-            const uint16_t* src = p.v + (int64_t)(w.tok0 + key) * p.ldv + w.head * H + i * 32;
+            const uint16_t* src = p.v + (int64_t)(w.tok0 + key) * p.ldv + w.head[x] * H + i * 32;
 #pragma unroll
             for (int k = 0; k < 32; k++) {
               const uint16_t e = src[k];
