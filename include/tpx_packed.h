@@ -79,7 +79,7 @@ int tpx_int4_attention(const TpxInt4Attention* a, void* stream);
 
 /* Attention over whole prompts: softmax(q k^T * scale) v for the T rows q [T][Nq][H], k and v [T][Nkv][H] (ld* elements apart, heads
  * side by side, 16-byte aligned), each within its sequence; causal: token i of a sequence sees the keys 0 .. i. Only the rows of
- * sequences are written to out [T][Nq][H]. H 64 or 128, at most 128 query heads per key head. Values that a row does not see
+ * sequences are written to out [T][Nq][H]. H 64 or 128, at most 128 query heads per key head, scale > 0. Values that a row does not see
  * never reach it, infinities and NaN included. Waits inside the kernel are bounded: tpx_packed_status reads and clears the code of one that gave up. */
 typedef struct {
   const uint16_t *q, *k, *v;

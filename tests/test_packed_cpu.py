@@ -128,7 +128,8 @@ def packed(**kw):
 
 @pytest.mark.parametrize("kw,rc", [(dict(q=None), 1), (dict(v=None), 1), (dict(cu_seqlens=None), 1), (dict(out=None), 1), (dict(H=96), 2), (dict(H=256), 2), (dict(Nq=5), 1),
                                    (dict(Nkv=0), 1), (dict(Nq=258), 2), (dict(B=0), 1), (dict(T=-1), 1), (dict(T=1 << 31), 1), (dict(k=A + 8), 1), (dict(ldv=260), 1),
-                                   (dict(T=1 << 30, Nkv=4), 1)])
+                                   (dict(T=1 << 30, Nkv=4), 1),
+                                   (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1)])
 def test_packed_attention_refuses(kw, rc):
     assert packed(**kw) == rc and lib().tpx_last_error()
     assert packed(T=0, q=None) == 0

@@ -137,6 +137,6 @@ def attention_int4(q, cache, layer, cu_seqlens=None, causal=True, scale=None, ou
 
 def attention_packed(q, k, v, cu_seqlens, causal=True, scale=None, out=None):
     """Attention over whole prompts laid end to end: q bf16 [T, heads, H], k and v [T, kv_heads, H] (rows may be strided, as views of a
-    q/k/v linear's output are; H 64 or 128; up to 128 heads per key head): softmax(q k^T scale) v within each sequence, where token i
+    q/k/v linear's output are; H 64 or 128; up to 128 heads per key head; scale > 0, H^-1/2 by default): softmax(q k^T scale) v within each sequence, where token i
     sees the tokens 0 .. i, or with causal=False all of them. bf16 [T, heads, H]; rows of no sequence are not written."""
     return _lib.torch_ops().packed_attention(q, k, v, cu_seqlens, causal, scale, out)

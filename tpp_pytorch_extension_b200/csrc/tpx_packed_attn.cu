@@ -125,28 +125,6 @@ __device__ __forceinline__ f32x2 pk_mul2(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of a pair without the special-function unit: x = n + f with n the nearest whole number (1.5 * 2^23 brings it to the low bits), a polynomial of degree 4
-// in f, -1/2 <= f <= 1/2, with the smallest relative error (2.6e-6, fitted for this kernel), and n added to its exponent. x below -126 gives
-// 2^-126 or so in the place of less.
-__device__ __forceinline__ f32x2 pk_exp2_pair(f32x2 x) {
-  float a, b;
-  pk_halves(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
-  x = pk_pair(a, b);
-  const f32x2 big = pk_pair(12582912.0f, 12582912.0f), t = pk_add2(x, big), n = pk_add2(t, pk_pair(-12582912.0f, -12582912.0f));
-  const f32x2 f = pk_fma2(n, pk_pair(-1.0f, -1.0f), x);
-  f32x2 y = pk_fma2(pk_pair(0.009570101276040077f, 0.009570101276040077f), f, pk_pair(0.05591785907745361f, 0.05591785907745361f));
-  y = pk_fma2(y, f, pk_pair(0.240247443318367f, 0.240247443318367f));
-  y = pk_fma2(y, f, pk_pair(0.6931217908859253f, 0.6931217908859253f));
-  y = pk_fma2(y, f, pk_pair(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb;
-  pk_halves(t, ta, tb);
-  pk_halves(y, a, b);
-  a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
-  b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
-  return pk_fma2(f, 0, pk_pair(a, b));  // a NaN, which the addition to the exponent has undone
-}
 __device__ __forceinline__ uint32_t pk_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -216,7 +194,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                    const PkParams p) {
   using C = PkCfg<H>;
   extern __shared__ unsigned char pk_smem_raw[];
-  __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], o_free[2], kv_full[C::SLOTS], kv_empty[C::SLOTS];
+  __shared__ __align__(8) unsigned long long q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_free[2], kv_full[C::SLOTS], kv_empty[C::SLOTS];
   __shared__ uint32_t tmem_holder;
   __shared__ int dirty;  // some value in a tile's margin is not finite
   __shared__ int pre[kPkBuckets + 1], warp_sum[kPkThreads / 32];
@@ -231,7 +209,6 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       tc_mbar_init(tc_smem_u32(&q_full[x]), 1);
       tc_mbar_init(tc_smem_u32(&q_empty[x]), 1);
       tc_mbar_init(tc_smem_u32(&s_full[x]), 1);
-      tc_mbar_init(tc_smem_u32(&p_half[x]), 128);
       tc_mbar_init(tc_smem_u32(&p_full[x]), 128);
       tc_mbar_init(tc_smem_u32(&o_full[x]), 1);
       tc_mbar_init(tc_smem_u32(&o_free[x]), 128);
@@ -355,11 +332,11 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       };
       auto scores = [&](int x, int slot) {
         tc_fence_after();
-        const uint32_t q0 = q_s + x * C::TILE_BYTES, k0 = kv_s + slot * C::TILE_BYTES;
+        const uint64_t q0 = tc_smem_desc(q_s + x * C::TILE_BYTES), k0 = tc_smem_desc(kv_s + slot * C::TILE_BYTES);
 #pragma unroll
         for (int kk = 0; kk < H / 16; kk++) {
-          const uint32_t off = (uint32_t)(kk >> 2) * C::HALF_BYTES + (uint32_t)(kk & 3) * 32;
-          pk_mma_ss(tmem + C::COL_S + x * 128, tc_smem_desc(q0 + off), tc_smem_desc(k0 + off), idesc_s, kk > 0 ? 1u : 0u);
+          const uint64_t off = (uint64_t)((kk >> 2) * (C::HALF_BYTES / 16) + (kk & 3) * 2);
+          pk_mma_ss(tmem + C::COL_S + x * 128, q0 + off, k0 + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         tc_commit(tc_smem_u32(&s_full[x]));
       };
@@ -397,15 +374,13 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
               if (!wait(&kv_full[vs], c / C::SLOTS)) break;
             }
             if (j == 0 && seen[x] && !wait(&o_free[x], seen[x] - 1)) break;
-            for (int half = 0; ok && half < 2; half++) {  // weights of the first, of the last 64 keys
-              if (!wait(half ? &p_full[x] : &p_half[x], steps[x])) break;
-              tc_fence_after();
+            if (!wait(&p_full[x], steps[x])) break;
+            tc_fence_after();
+            const uint64_t v0 = pk_desc_mn(kv_s + vs * C::TILE_BYTES, C::HALF_BYTES);
 #pragma unroll
-              for (int kk = half * 4; kk < half * 4 + 4; kk++)  // 16 keys: 8 columns of packed weights, two 8-key groups of values
-                pk_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + kk * 8, pk_desc_mn(kv_s + vs * C::TILE_BYTES + kk * 2048, C::HALF_BYTES), idesc_o,
-                          j > 0 || kk > 0 ? 1u : 0u);
-            }
-            if (!ok) break;
+            for (int kk = 0; kk < 8; kk++)  // 16 keys: 8 columns of packed weights, two 8-key groups of values
+              pk_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + kk * 8, v0 + kk * 128, idesc_o,
+                        j > 0 || kk > 0 ? 1u : 0u);
             steps[x]++;
             if (j + 1 < w.tiles[x]) {
               scores(x, ks);
@@ -455,8 +430,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       const bool live = tok < p.TPT && t < w.n;
       const int klim = p.causal ? min(t + 1, w.n) : w.n;               // keys [0, klim) are seen (dead rows: anything)
       const int whole = (p.causal ? w.t0[0] + 1 : w.n) / 128;              // key tiles that every row of the unit sees in full
-      float m_ref = -INFINITY, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      f32x2 l2[2] = {0, 0};  // two more pairs of partial sums
+      float m_ref = -INFINITY;
+      f32x2 l2[2] = {0, 0};  // partial sums of the weights
       for (int j = 0; j < n; j++) {
         if (!wait(&s_full[x], steps)) break;
         steps++;
@@ -471,20 +446,17 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           const int lim = klim - j * 128;
 #pragma unroll
           for (int i = 0; i < 128; i++)
-            if (i >= lim) s[i] = p.sc2 < 0.0f ? INFINITY : -INFINITY;
+            if (i >= lim) s[i] = -INFINITY;
         }
         float unit = p.sc2;
-        if (!(unit > 0.0f)) {  // the scale does not keep the order: scores take it first
+        float top8[8];
 #pragma unroll
-          for (int i = 0; i < 128; i++) s[i] = margin && i >= klim - j * 128 ? -INFINITY : s[i] * unit;
-          unit = 1.0f;
-        }
-        float top4[4] = {s[0], s[1], s[2], s[3]};
+        for (int k = 0; k < 8; k++) top8[k] = fmaxf(pk_max3(s[2 * k], s[2 * k + 1], s[16 + 2 * k]), s[17 + 2 * k]);
 #pragma unroll
-        for (int i = 4; i < 124; i += 8)
+        for (int i = 32; i < 128; i += 16)
 #pragma unroll
-          for (int k = 0; k < 4; k++) top4[k] = pk_max3(top4[k], s[i + 2 * k], s[i + 2 * k + 1]);
-        float top = pk_max3(pk_max3(top4[0], top4[1], top4[2]), pk_max3(top4[3], s[124], s[125]), fmaxf(s[126], s[127]));
+          for (int k = 0; k < 8; k++) top8[k] = pk_max3(top8[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        float top = fmaxf(pk_max3(pk_max3(top8[0], top8[1], top8[2]), top8[3], top8[4]), pk_max3(top8[5], top8[6], top8[7]));
         // The multiply-add below takes the rounded reference off an unrounded score, which is nothing for ordinary scores; large ones are
         // rounded first, so that the largest weight is what it should be
         if (__any_sync(0xffffffffu, !(fabsf(top) * unit < 4096.0f)) && unit != 1.0f) {
@@ -498,8 +470,6 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (__any_sync(0xffffffffu, pass)) {
           const float m_new = pass ? top : m_ref, alpha = pass ? pk_ex2(m_ref - m_new) : 1.0f;
           m_ref = m_new;
-#pragma unroll
-          for (int i = 0; i < 4; i++) l[i] *= alpha;
           l2[0] = pk_mul2(l2[0], pk_pair(alpha, alpha));
           l2[1] = pk_mul2(l2[1], pk_pair(alpha, alpha));
           if (j > 0) {
@@ -546,39 +516,16 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           uint32_t pw[32];
-          if (margin) {
 #pragma unroll
-            for (int k = 0; k < 32; k++) {
-              const float a = pk_ex2(fmaf(s[64 * i + 2 * k], unit, -ref)), b = pk_ex2(fmaf(s[64 * i + 2 * k + 1], unit, -ref));
-              l[k & 3] += a + b;
-              pw[k] = pk_pack(a, b);
-            }
-          } else {
-            // the special-function unit is as busy as the tensor core (16 of 2^x, 8192 products per clock): every third pair goes to the multiply-adds
-#pragma unroll
-            for (int k = 0; k < 32; k++) {
-              f32x2 e = pk_fma2(pk_pair(s[64 * i + 2 * k], s[64 * i + 2 * k + 1]), unit2, ref2);
-              float a, b;
-              if (k % 3 == 2) {
-                e = pk_exp2_pair(e);
-                pk_halves(e, a, b);
-              } else {
-                pk_halves(e, a, b);
-                a = pk_ex2(a);
-                b = pk_ex2(b);
-                e = pk_pair(a, b);
-              }
-              l2[k & 1] = pk_add2(l2[k & 1], e);
-              pw[k] = pk_pack(a, b);
-            }
+          for (int k = 0; k < 32; k++) {
+            float a, b;
+            pk_halves(pk_fma2(pk_pair(s[64 * i + 2 * k], s[64 * i + 2 * k + 1]), unit2, ref2), a, b);
+            a = pk_ex2(a);
+            b = pk_ex2(b);
+            l2[k & 1] = pk_add2(l2[k & 1], pk_pair(a, b));
+            pw[k] = pk_pack(a, b);
           }
           pk_st32(s_t + i * 32, pw);
-          if (i == 0) {
-            __syncwarp();
-            pk_st_wait();
-            tc_fence_before();
-            tc_mbar_arrive(tc_smem_u32(&p_half[x]));
-          }
         }
         __syncwarp();
         pk_st_wait();
@@ -588,10 +535,10 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
       if (!wait(&o_full[x], seen)) break;
       seen++;
       tc_fence_after();
-      float more[4];
-      pk_halves(l2[0], more[0], more[1]);
-      pk_halves(l2[1], more[2], more[3]);
-      const float inv = 1.0f / (((l[0] + l[1]) + (l[2] + l[3])) + ((more[0] + more[1]) + (more[2] + more[3])));
+      float l[4];
+      pk_halves(l2[0], l[0], l[1]);
+      pk_halves(l2[1], l[2], l[3]);
+      const float inv = 1.0f / ((l[0] + l[1]) + (l[2] + l[3]));
       const bool mend = *reinterpret_cast<volatile int*>(&dirty) != 0;
       uint16_t* dst = p.out + ((int64_t)(w.tok0 + (live ? t : 0)) * p.Nq + w.head[x] * p.R + member) * H;
 #pragma unroll
@@ -691,6 +638,7 @@ extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) {
               "packed_attention: %ld tokens of %ld sequences", (long)a->T, (long)a->B);
   TPX_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) & 15) == 0 && (a->ldq | a->ldk | a->ldv) % 8 == 0, TPX_ERR_ARG,
               "packed_attention: tensors and their rows must be 16-byte aligned");
+  TPX_REQUIRE(a->scale > 0.0f && a->scale < INFINITY, TPX_ERR_ARG, "packed_attention: a scale of %g (it must be positive)", (double)a->scale);
   if (a->T == 0) return TPX_OK;
   PkParams p = {};
   p.cu = a->cu_seqlens;
