@@ -509,6 +509,34 @@ class LlamaDecoderLayer:
         return [out]
 
 
+    def forward_packed(self, hs, cache, cu_seqlens=None, positions=None):
+        """The same layer for sequences laid end to end without padding, on a cache that is held in 4 bits: hs bf16 [T, D],
+        cache a _packed_attn.Int4Cache with pages for the new tokens (this layer's keys and values go into it; its lengths
+        stay, Int4Cache.advance() moves them after the last layer).
+
+        With cu_seqlens (int32 [B + 1]) the call holds whole prompts, the first tokens of sequences that have nothing
+        cached, and attention runs over their keys and values before they are quantized. Without it row b is the next
+        token of sequence b, and attention reads the cache. positions (int64 [T]): rows of the rotary table, by default the
+        tokens' places in their sequences. Returns [T, D]."""
+        from . import _packed_attn as P
+        _lib.require_cuda(hs, "hidden_states")
+        T, ws = hs.shape[0], get_pg_size()
+        qkv = fc_plain_norm(hs, self.Gi, self.eps, self.Wqkv, self.Bqkv)
+        q, k = P.qk_norm_rope(qkv, self.Nq, self.Nkv, self.H, ep=self.EP, positions=positions, cu_seqlens=cu_seqlens, cache=cache,
+                              layer=self.layer_idx, want_k=cu_seqlens is not None)
+        if cu_seqlens is None:
+            ctx = P.attention_int4(q, cache, self.layer_idx)
+        else:
+            v = qkv[:, (self.Nq + self.Nkv) * self.H:].view(T, self.Nkv, self.H)
+            ctx = P.attention_packed(q, k, v, cu_seqlens)
+        so = fc_plain_act(ctx.view(T, self.Nq * self.H), self.Wp, res=hs, res_scale=1.0 / ws)
+        if ws > 1:
+            allreduce(so)
+        out = fc_plain_act(fc_gate_up(so, self.Wg, self.Wu, "silu", norm=(self.Gpa, self.eps)), self.Wd, res=so, res_scale=1.0 / ws)
+        if ws > 1:
+            allreduce(out)
+        return out
+
     # ----- the same forward as two C calls (tpx_llama_layer_attention / tpx_llama_layer_mlp): one foreign call per half
     # of the layer instead of one per kernel
     def _c_level_ok(self):

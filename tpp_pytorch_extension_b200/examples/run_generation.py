@@ -44,6 +44,7 @@ def main(argv=None):
     ap.add_argument("--num-warmup", type=int, default=1)
     ap.add_argument("--layers", type=int, default=0, help="keep only this many decoder layers (0 = all)")
     ap.add_argument("--no-graph", action="store_true", help="decode eagerly instead of replaying a CUDA graph")
+    ap.add_argument("--kv-cache", default="bfloat16", choices=["bfloat16", "int4"], help="int4: prompts without padding on a cache held in 4 bits (Llama and Qwen2 layers)")
     ap.add_argument("--quantize-lm-head", action="store_true", help="quantize the lm_head like the decoder linears (bf16 otherwise)")
     ap.add_argument("--save-sharded-model", action="store_true", help="write this rank's quantized, packed shard to ./sharded_model/r<rank>_<size>/model.pt")
     ap.add_argument("--load-sharded-model", action="store_true", help="read the shard written by --save-sharded-model instead of building the model")
@@ -92,7 +93,10 @@ def main(argv=None):
     def run(new):
         torch.cuda.synchronize()
         t0 = time.perf_counter()
-        out = model.generate(ids, new, use_graph=not a.no_graph)
+        if a.kv_cache == "int4":
+            out = model.generate_packed(list(ids), new, use_graph=not a.no_graph)
+        else:
+            out = model.generate(ids, new, use_graph=not a.no_graph)
         torch.cuda.synchronize()
         return time.perf_counter() - t0, out
 
@@ -111,7 +115,7 @@ def main(argv=None):
         print(json.dumps({
             "model": a.model, "weight_dtype": a.dtype if isinstance(shape, HYBRID) else a.weight_dtype, "tp": world, "layers": shape.num_hidden_layers,
             "batch_size": a.batch_size, "input_tokens": a.input_tokens, "max_new_tokens": a.max_new_tokens,
-            "graph": not a.no_graph, "first_token_ms": round(t1 * 1e3, 3), "next_token_ms": round(per_tok * 1e3, 4),
+            "graph": not a.no_graph, "kv_cache": a.kv_cache, "first_token_ms": round(t1 * 1e3, 3), "next_token_ms": round(per_tok * 1e3, 4),
             "decode_tokens_per_s": round(a.batch_size / per_tok, 1),
             "prefill_tokens_per_s": round(a.batch_size * a.input_tokens / t1, 1), "data": "synthetic"}))
     if world > 1:

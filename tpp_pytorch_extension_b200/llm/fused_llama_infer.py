@@ -285,6 +285,59 @@ class LlamaRunner(torch.nn.Module):
         return out
 
     @torch.no_grad()
+    def generate_packed(self, prompts, max_new_tokens, use_graph=True):
+        """Greedy decoding of prompts of unequal lengths, a list of int64 [tokens] on the device, without padding: the prompts
+        run laid end to end, every sequence then gets one token per step, and keys and values are cached in 4 bits
+        (_packed_attn.Int4Cache: 9 / 32 of what bf16 pages hold). Head sizes 64 and 128. As in generate(), use_graph records
+        the step once and replays it. Returns a list of [tokens + max_new_tokens]."""
+        from .. import _lib
+        from .._C._packed_attn import Int4Cache
+        layers = getattr(self, "layers", None)
+        if not layers or not all(hasattr(layer, "forward_packed") for layer in layers):
+            raise _lib.TpxError("generate_packed: the layers of this model have no packed form")
+        if not prompts or any(p.dim() != 1 or not p.numel() for p in prompts) or max_new_tokens < 1:
+            raise _lib.TpxError("generate_packed: prompts are a list of one-dimensional, not empty tensors, and one new token is the least")
+        lens = [p.numel() for p in prompts]
+        total = [n + max_new_tokens - 1 for n in lens]  # cached in the end: the last new token is not
+        B, dev, first = len(prompts), prompts[0].device, layers[0]
+        if max(total) > first.EP.shape[1]:
+            raise _lib.TpxError(f"generate_packed: {max(total)} tokens pass the {first.EP.shape[1]} positions of the rotary table")
+        cache = Int4Cache(len(layers), sum(-(-n // 32) for n in total), first.Nkv, first.H, B, -(-max(total) // 32), dev)
+        cache.add_pages(total)
+        cu = torch.tensor([0] + lens).cumsum(0).to(dev, torch.int32)
+        pos = torch.cat([torch.arange(n) for n in lens]).to(dev)
+
+        def run(ids, pos, cu):  # the next token of every sequence, [B, 1]
+            hs = self._embed(ids, pos).view(ids.shape[1], -1)
+            for layer in layers:
+                hs = layer.forward_packed(hs, cache, cu, pos.view(-1))
+            cache.advance(cu)
+            rows = hs if cu is None else hs[cu[1:].long() - 1]
+            return self._pick(self._head(rows.unsqueeze(1)))
+
+        tok = run(torch.cat(list(prompts)).unsqueeze(0), pos.unsqueeze(0), cu)
+        pos = torch.tensor(lens, device=dev).unsqueeze(0)
+
+        def step():
+            tok.copy_(run(tok.view(1, B), pos, None))
+            pos.add_(1)
+
+        outs, graph = [tok.clone()], None
+        while len(outs) < max_new_tokens:
+            if graph is not None:
+                graph.replay()
+            else:
+                step()
+                if use_graph and max_new_tokens - len(outs) > 2:  # the first step ran eagerly: scratch has its size
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        step()
+            outs.append(tok.clone())
+        _lib.assert_no_kernel_error()
+        new = torch.cat(outs, dim=1)
+        return [torch.cat([p, n]) for p, n in zip(prompts, new)]
+
+    @torch.no_grad()
     def beam_search(self, input_ids, max_new_tokens, num_beams=4, attention_mask=None):
         """Beam search for a fixed number of new tokens (the reference's default driver runs Hugging Face generate with
         num_beams=4, examples/llm/run_generation.py:337-339; its own part is the cache reordering, which this uses).
