@@ -311,6 +311,30 @@ def test_nan_and_infinity_reach_those_who_see_them():
         assert out[3 * b + 1].isnan().all() and out[3 * b + 2].isnan().all()  # the infinity; the NaN too
 
 
+@pytest.mark.parametrize("old", [[0, 40], [5000, 0], [20000, 3], [3] * 300])
+@pytest.mark.parametrize("what", ["query", "keys"])
+def test_scores_that_are_all_nan_give_nan(what, old):
+    """A row whose every score is a NaN has no largest score, but it is not a row without keys: by one warp, a block and many blocks."""
+    g, H = gen(23, len(old), old[0]), 64
+    n = len(old)
+    cache = new_cache(old, [1] * n, 2, H, g)
+    k, v = (rand(g, sum(old) + n, 2, H).bfloat16() for _ in range(2))
+    q = rand(g, n, 4, H).bfloat16()
+    cu = cu_of([m + 1 for m in old])
+    if what == "query":
+        q[0, 1, 7] = math.nan
+    else:
+        k[:int(cu[1]), 0] = math.nan
+    start = cache.lengths.clone()
+    cache.lengths.zero_()
+    P().append_int4(k, v, cache, 0, cu)
+    cache.lengths.copy_(start)
+    out = P().attention_int4(q, cache, 0)
+    bad = torch.zeros((n, 4), dtype=torch.bool, device="cuda")
+    bad[0, 1 if what == "query" else slice(0, 2)] = True
+    assert torch.equal(out.isnan().all(-1), bad) and bool(out[~bad].isfinite().all())
+
+
 def test_offsets_behind_two_gigabytes():
     old, new, H = [100, 40], [1, 1], 128
     pages = 2 ** 31 // 4608 + 40
@@ -385,3 +409,40 @@ def test_empty_calls():
     assert P().read_int4(cache, 0, 0, cu)[0].shape == (0, 1, 64)
     q, k = P().qk_norm_rope(torch.empty(0, 3 * 64, device="cuda", dtype=torch.bfloat16), 1, 1, 64)
     assert q.shape == (0, 1, 64)
+
+
+def test_refused_tensors():
+    """What the host sees of a call that cannot work: none of these launches anything."""
+    from tpp_pytorch_extension_b200._lib import TpxError
+    g, old = gen(31), [40, 0]
+    cache = new_cache(old, [1, 1], 2, 64, g)
+    qkv = rand(g, 2, 8 * 64).bfloat16()
+    q, k = qkv[:, :256].contiguous().view(2, 4, 64), qkv[:, 256:384].contiguous().view(2, 2, 64)
+    ep = table(64, 64)
+    prep = lambda x=qkv, **kw: P().qk_norm_rope(x, 4, 2, 64, ep=ep, cache=cache, **kw)  # noqa: E731
+    cu = cu_of([1, 1])
+    refused = [
+        lambda: prep(qkv.cpu()), lambda: prep(qkv.float()), lambda: prep(qkv[:, :448]), lambda: prep(qkv[:1]), lambda: prep(qkv.clone().requires_grad_()),
+        lambda: prep(q_out=qkv[:, :256].view(2, 4, 64)), lambda: prep(q_out=torch.empty_like(q).float()), lambda: prep(q_out=torch.empty_like(k)),
+        lambda: prep(q_out=qkv.view(-1)[:512].view(2, 4, 64)), lambda: prep(q_out=q, k_out=q.view(-1)[:256].view(2, 2, 64)),
+        lambda: prep(positions=torch.zeros(2, dtype=torch.int32, device="cuda")), lambda: prep(positions=torch.zeros(3, dtype=torch.int64, device="cuda")),
+        lambda: prep(q_norm=torch.ones(64, device="cuda"), k_norm=torch.ones(64, device="cuda").bfloat16()), lambda: prep(q_norm=torch.ones(32, device="cuda")),
+        lambda: prep(cu_seqlens=cu.long()), lambda: prep(cu_seqlens=cu[:2]),
+        lambda: P().qk_norm_rope(qkv, 4, 2, 64, ep=ep), lambda: P().qk_norm_rope(qkv, 4, 2, 64, cu_seqlens=cu),
+        lambda: P().qk_norm_rope(qkv, 8, 4, 32, cache=cache), lambda: P().qk_norm_rope(qkv, 2, 3, 64, cache=cache),
+        lambda: P().append_int4(k, k[:1], cache, 0), lambda: P().append_int4(k[:, :1], k[:, :1], cache, 0), lambda: P().append_int4(k.float(), k.float(), cache, 0),
+        lambda: P().append_int4(k.transpose(0, 1), k.transpose(0, 1), cache, 0), lambda: P().append_int4(k[:1], k[:1], cache, 0),
+        lambda: P().read_int4(cache, 0, 3), lambda: P().read_int4(cache, 0, 2, lengths=cu), lambda: P().read_int4(cache, 0, -1),
+        lambda: P().attention_int4(q[:, :3], cache, 0), lambda: P().attention_int4(q[:1], cache, 0), lambda: P().attention_int4(q.float(), cache, 0),
+        lambda: P().attention_int4(q, cache, 0, scale=math.inf), lambda: P().attention_int4(q, cache, 0, scale=math.nan),
+        lambda: P().attention_int4(q, cache, 0, out=q), lambda: P().attention_int4(q, cache, 0, out=cache.pools[0].view(-1)[:1024].view(torch.bfloat16).view(2, 4, 64)),
+        lambda: P().attention_int4(q.expand(2, 4, 64)[:, :, ::2], cache, 0), lambda: P().attention_int4(q.detach().requires_grad_(), cache, 0),
+    ]
+    before = cache.pools[0].clone()
+    for i, call in enumerate(refused):
+        with pytest.raises(TpxError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert torch.equal(before, cache.pools[0])
+    with torch.no_grad():  # leaves that want a gradient may be used where none is recorded
+        P().attention_int4(q.clone().requires_grad_(), cache, 0)

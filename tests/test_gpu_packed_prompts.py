@@ -187,3 +187,37 @@ def test_streams_graphs_and_repetition():
 def test_empty_call():
     q = torch.empty(0, 4, 64, device="cuda", dtype=torch.bfloat16)
     assert P().attention_packed(q, q[:, :2], q[:, :2], cu_of([0, 0])).shape == (0, 4, 64)
+
+
+def test_refused_tensors():
+    from tpp_pytorch_extension_b200._lib import TpxError
+    q, k, v = inputs(gen(41), 9, 4, 2, 64)
+    cu = cu_of([5, 4])
+    A = P().attention_packed
+    refused = [
+        lambda: A(q, k, v, None), lambda: A(q, k, v, cu.long()), lambda: A(q, k, v, cu[:1]), lambda: A(q, k, v, cu.cpu()), lambda: A(q.cpu(), k, v, cu),
+        lambda: A(q[:8], k, v, cu), lambda: A(q[:, :3], k, v, cu), lambda: A(q, k, v[:, :1], cu), lambda: A(q, k[..., :32], v[..., :32], cu),
+        lambda: A(q[..., :32], k[..., :32], v[..., :32], cu), lambda: A(q.float(), k.float(), v.float(), cu), lambda: A(q.half(), k.half(), v.half(), cu),
+        lambda: A(q, k, v, cu, scale=0.0), lambda: A(q, k, v, cu, scale=-1.0), lambda: A(q, k, v, cu, scale=math.nan), lambda: A(q, k, v, cu, scale=math.inf),
+        lambda: A(q, k, v, cu, out=q), lambda: A(q, k, v, cu, out=torch.empty_like(k)), lambda: A(q, k, v, cu, out=torch.empty_like(q).float()),
+        lambda: A(q, k, v, cu, out=torch.empty(9, 8, 64, device="cuda", dtype=torch.bfloat16)[:, ::2]), lambda: A(q.clone().requires_grad_(), k, v, cu),
+        lambda: A(q, k.transpose(0, 1), v.transpose(0, 1), cu), lambda: A(q, k[:1].expand(9, 2, 64), v, cu),
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(TpxError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    assert_no_kernel_error()
+
+
+def test_a_sequence_does_not_feel_its_neighbours():
+    """Rows of other sequences in a tile, whatever their scores are, change no bit."""
+    g = gen(43)
+    q, k, v = inputs(g, 330, 7, 1, 128)
+    cu = cu_of([200, 130])
+    plain = P().attention_packed(q, k, v, cu)
+    q2, k2, v2 = q.clone(), k.clone(), v.clone()
+    for t, x in ((q2, 2.0 ** 40), (k2, -2.0 ** 40), (v2, math.inf)):
+        t[200:] = x
+    assert torch.equal(P().attention_packed(q2, k2, v2, cu)[:200], plain[:200])
+    assert_no_kernel_error()

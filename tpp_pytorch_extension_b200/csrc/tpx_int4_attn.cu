@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 #pragma unroll
       for (int j = 0; j < RT; j++) {
         if (4 * j + t >= rows) continue;
-        const float inv = m_run[j] == -INFINITY ? 0.0f : 1.0f / l_run[j];
+        const float inv = l_run[j] == 0.0f ? 0.0f : 1.0f / l_run[j];  // 0: no keys
         uint16_t* dst = row_out(4 * j + t);
 #pragma unroll
         for (int h = 0; h < G; h++) {
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
             }
 #pragma unroll
             for (int j = 0; j < RT; j++) {
-              if (pm[j] == -INFINITY) continue;  // saw nothing of this row
+              if (pl[j] == 0.0f) continue;  // saw nothing of this row (scores that are all NaN leave the maximum behind, but a sum)
               const float m_new = fmaxf(m_run[j], pm[j]), fo = i4_ex2(m_run[j] - m_new), fn = i4_ex2(pm[j] - m_new);
               m_run[j] = m_new;
               l_run[j] = fmaf(l_run[j], fo, pl[j] * fn);
@@ -787,8 +787,8 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
       }
       group_sync();
       float* part = part_of(me);
-      auto store = [&](int r, int d, float m, float l, const float4& v) {
-        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+      auto store = [&](int r, int d, float l, const float4& v) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         *reinterpret_cast<uint2*>(row_out(r) + d) = make_uint2(i4_pack_bf16(v.x * inv, v.y * inv), i4_pack_bf16(v.z * inv, v.w * inv));
       };
       auto add = [&](float4& v, float fo, const float4& x, float fn) {
@@ -806,14 +806,14 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < GW; k++) {
           const float* from = reinterpret_cast<const float*>(group_base + k * C::WARP_BYTES);
-          const float pm = from[ROWS * C::PITCH + r];
-          if (pm == -INFINITY) continue;  // a warp that saw nothing of this row
+          const float pm = from[ROWS * C::PITCH + r], pl = from[ROWS * C::PITCH + ROWS + r];
+          if (pl == 0.0f) continue;  // a warp that saw nothing of this row
           const float f = i4_ex2(pm - ref);
-          l = fmaf(from[ROWS * C::PITCH + ROWS + r], f, l);
+          l = fmaf(pl, f, l);
           add(v, 1.0f, *reinterpret_cast<const float4*>(from + r * C::PITCH + d), f);
         }
         if (whole) {
-          store(r, d, m, l, v);
+          store(r, d, l, v);
         } else {
           reinterpret_cast<float4*>(part)[e] = v;
           if (d == 0) {
@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
               }
 #pragma unroll
               for (int k = 0; k < U; k++) {
-                if (k0 + k * splits > w1 || pm[k] == -INFINITY) continue;
+                if (k0 + k * splits > w1 || pl[k] == 0.0f) continue;
                 const float m_new = fmaxf(m, pm[k]), fo = i4_ex2(m - m_new), fn = i4_ex2(pm[k] - m_new);
                 m = m_new;
                 l = fmaf(l, fo, pl[k] * fn);
@@ -864,14 +864,14 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
               if (first > 0) break;
               for (int k = 1; k < splits; k++) {
                 const float* from = reinterpret_cast<const float*>(group_base + (w + k * (ITEMS / 32)) * C::WARP_BYTES) + lane * 6;
-                if (from[0] == -INFINITY) continue;
+                if (from[1] == 0.0f) continue;
                 const float m_new = fmaxf(m, from[0]), fo = i4_ex2(m - m_new), fn = i4_ex2(from[0] - m_new);
                 m = m_new;
                 l = fmaf(l, fo, from[1] * fn);
                 add(v, fo, make_float4(from[2], from[3], from[4], from[5]), fn);
               }
             }
-            if (r < rows) store(r, d, m, l, v);
+            if (r < rows) store(r, d, l, v);
           }
         }
       }
@@ -924,6 +924,7 @@ extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
               (long)a->cache->B);
   TPX_REQUIRE(a->Nq > 0 && a->Nq <= 4096 && a->Nq % Nkv == 0, TPX_ERR_ARG, "int4_attention: %ld query heads for %ld key heads", (long)a->Nq, (long)Nkv);
   TPX_REQUIRE((((uintptr_t)a->q | (uintptr_t)a->out) & 15) == 0 && a->ldq % 8 == 0, TPX_ERR_ARG, "int4_attention: q, its rows and out must be 16-byte aligned");
+  TPX_REQUIRE(a->scale - a->scale == 0.0f, TPX_ERR_ARG, "int4_attention: a scale of %g", (double)a->scale);
   if (a->T == 0) return TPX_OK;
   const int rt = i4_rows(a->T, a->cache->B, a->Nq, Nkv);
   TPX_REQUIRE(a->scratch && ((uintptr_t)a->scratch & 255) == 0 && a->scratch_bytes >= i4_scratch(rt, H), TPX_ERR_SCRATCH,

@@ -458,8 +458,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
           for (int k = 0; k < 8; k++) top8[k] = pk_max3(top8[k], s[i + 2 * k], s[i + 2 * k + 1]);
         float top = fmaxf(pk_max3(pk_max3(top8[0], top8[1], top8[2]), top8[3], top8[4]), pk_max3(top8[5], top8[6], top8[7]));
         // The multiply-add below takes the rounded reference off an unrounded score, which is nothing for ordinary scores; large ones are
-        // rounded first, so that the largest weight is what it should be
-        if (__any_sync(0xffffffffu, !(fabsf(top) * unit < 4096.0f)) && unit != 1.0f) {
+        // rounded first, so that the largest weight is what it should be (for all rows of a warp, so rows of no token have no say in it)
+        if (__any_sync(0xffffffffu, live && !(fabsf(top) * unit < 4096.0f)) && unit != 1.0f) {
 #pragma unroll
           for (int i = 0; i < 128; i++) s[i] *= unit;
           top *= unit;

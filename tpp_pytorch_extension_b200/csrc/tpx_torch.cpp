@@ -53,6 +53,18 @@ struct Call {
   const char* name;
   PyObject* const* args;
   c10::DeviceIndex device = -1;  // of the tensors so far
+  struct { uintptr_t from, to; } spans[12];  // memory of the arguments so far: an output may lie over none
+  int spans_n = 0;
+
+  void note(const void* from, int64_t bytes) {
+    if (bytes > 0) spans[spans_n++] = {(uintptr_t)from, (uintptr_t)from + (uintptr_t)bytes};
+  }
+  static int64_t extent(const at::Tensor& t) {
+    if (t.numel() == 0) return 0;
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); i++) last += (t.size(i) - 1) * t.stride(i);
+    return (last + 1) * (int64_t)t.element_size();
+  }
 
   void on(const at::Tensor& t, const char* what) {
     if (!t.is_cuda()) refuse("%s: %s must be on a CUDA device (this library has no CPU path)", name, what);
@@ -69,6 +81,7 @@ struct Call {
     if (!THPVariable_Check(args[i])) refuse("%s: %s must be a tensor", name, what);
     const at::Tensor& t = THPVariable_Unpack(args[i]);
     on(t, what);
+    note(t.data_ptr(), extent(t));
     return t;
   }
   int64_t integer(int i, const char* what) {
@@ -109,8 +122,14 @@ struct Call {
   }
   at::Tensor output(int i, c10::IntArrayRef shape) {
     if (i < 0 || none(i)) return at::empty(shape, at::TensorOptions().dtype(at::kBFloat16).device(at::kCUDA, device));
-    const at::Tensor& t = tensor(i, "the output");
+    if (!THPVariable_Check(args[i])) refuse("%s: the output must be a tensor", name);
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    on(t, "the output");
     if (t.scalar_type() != at::kBFloat16 || t.sizes() != shape || !t.is_contiguous()) refuse("%s: the output must be contiguous bf16 of the result's shape", name);
+    const uintptr_t from = (uintptr_t)t.data_ptr(), to = from + (uintptr_t)extent(t);
+    for (int k = 0; k < spans_n; k++)
+      if (from < spans[k].to && spans[k].from < to) refuse("%s: the output overlaps another argument", name);
+    note(t.data_ptr(), extent(t));
     return t;
   }
   void* stream() { return (void*)c10::cuda::getCurrentCUDAStream(device).stream(); }
@@ -136,6 +155,9 @@ const TpxInt4Cache* cache_of(Call& c, int i) {
     if (b->device != now) refuse("%s: the cache is on cuda:%d, the current device is cuda:%d", c.name, (int)b->device, (int)now);
     c.device = now;
   }
+  c.note(b->c.pool, b->c.pages * b->c.kv_heads * 36 * b->c.H);
+  c.note(b->c.table, b->c.B * b->c.table_cols * 4);
+  c.note(b->c.lengths, b->c.B * 4);
   return &b->c;
 }
 
