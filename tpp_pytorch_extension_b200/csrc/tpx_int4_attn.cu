@@ -151,6 +151,9 @@ struct I4Cfg {
   static constexpr int STAGES = 2;
   static constexpr int WARP_SHIFT = RT < 4 ? 4 : 3, WARPS = 1 << WARP_SHIFT;
   static_assert(WARPS <= kI4Warps, "scratch");
+  // The run's place in the share, which its pages do not need, waits in shared memory while they are walked. With 8 rows it saves spills (64 sequences of up to
+  // 4096 tokens, 64/8 heads of 128: 38.1 -> 34.6 us); with 4 rows it costs more than it saves (one of 131072, 32/8 heads: 44.2 -> 45.9 us)
+  static constexpr bool PARK = RT == 2;
   static constexpr int TILES = RT + (RT + 1) / 2;          // n-tiles of q digits: upper two of 4 rows each, lowest of 8
   static constexpr int PITCH = H + 4;                      // floats of a row in the merge buffer
   static constexpr int MERGE = (ROWS * PITCH + 2 * ROWS) * 4;
@@ -167,6 +170,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   extern __shared__ __align__(16) unsigned char i4_smem[];
   __shared__ int scan[3][C::WARPS], start_off[C::WARPS];
   __shared__ int start_b[C::WARPS];
+  __shared__ int parked[C::WARPS][C::PARK ? 12 : 1];
   pdl_trigger();
   pdl_wait();
 
@@ -371,11 +375,10 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 
   int stage = 0;
   for (; now.b >= 0; next(now)) {
-    const int n_tok = i4_seq(p, now.b, ROWS).n, tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
-    const int w0 = (now.seg0 + start) / per, w1 = (now.seg0 + units_of(now.quanta) - 1) / per;  // the groups that share the segment
-    const bool whole = w0 == w1;
+    int n_tok = i4_seq(p, now.b, ROWS).n, tok0 = p.cu ? min(max(p.cu[now.b], 0), p.T) : now.b;
+    int w0 = (now.seg0 + start) / per, w1 = (now.seg0 + units_of(now.quanta) - 1) / per;  // the groups that share the segment
     unsigned long long word_was = 0;
-    if (!whole && gtid == 0) word_was = *reinterpret_cast<volatile unsigned long long*>(p.counters + w0);
+    if (w0 != w1 && gtid == 0) word_was = *reinterpret_cast<volatile unsigned long long*>(p.counters + w0);
     {  // the segment's query rows, as digits, by the group together
       constexpr int LR = H / 8;  // lanes per row
       uint2* frag = reinterpret_cast<uint2*>(group_base);
@@ -465,6 +468,12 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
           for (int i = 0; i < 4; i++) acc[v][h][i][0] = acc[v][h][i][1] = acc[v][h][i][2] = acc[v][h][i][3] = 0.0f;
     }
 
+    volatile int* const lot = parked[warp];
+    if (C::PARK && lane == 0) {
+      const int v[12] = {now.b, now.n, now.chunk, now.seg0, now.left, now.keys, now.quanta, now.chunks, tok0, n_tok, w0, w1};
+#pragma unroll
+      for (int i = 0; i < 12; i++) lot[i] = v[i];
+    }
     for (; now.qi < now.qend; now.qi++) {
     asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
     __syncwarp();
@@ -660,6 +669,12 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     }
 
     // ---- the run's end: rows of (maximum, sum, output); a lane has 8 dimensions 64 h + 8 g + .. of the rows 4 j + t
+    if (C::PARK) {
+      __syncwarp();
+      now = Run{lot[0], lot[1], lot[2], lot[3], now.qi, now.qend, lot[4], lot[5], lot[6], lot[7]};
+      tok0 = lot[8], n_tok = lot[9], w0 = lot[10], w1 = lot[11];
+    }
+    const bool whole = w0 == w1;
     const int rows = min(ROWS, n_tok * p.R - now.chunk * ROWS);
     // A part is [RT][G][2][32 lanes] float4 as the lanes have them, then maxima and sums; one of a share's first, one of its last segment
     auto part_of = [&](int k) { return p.part + ((int64_t)k * 2 + (now.seg0 + start < k * per ? 0 : 1)) * ROWS * (H + 2); };
