@@ -2,7 +2,7 @@
 q/k/v linear (head norms, rotation, append), attention over whole prompts and attention of a few new tokens over the cache, on the
 kernels of include/tpx_packed.h. They stand beside the padded batches and the bf16 pages of _tpp_attn.
 
-Token rows [T, ...] are cut into sequences by cu_seqlens (int32 [B + 1] on the device: sequence b has the rows cu[b] .. cu[b + 1] - 1);
+Token rows [T, ...] are cut into sequences by cu_seqlens (int32 [B + 1] on the device, not falling: sequence b has the rows cu[b] .. cu[b + 1] - 1);
 without it row b is the one token of sequence b. Rows outside every sequence are read by nobody, and an output that the caller
 passes has theirs left as they were. Nothing here waits for the device, so all of it can be recorded in a CUDA graph."""
 import torch
