@@ -161,6 +161,18 @@ def test_many_short_sequences():
     check(q, k, v, P().attention_packed(q, k, v, cu), lengths, cu, rows=set(range(0, 1500, 41)))
 
 
+@pytest.mark.parametrize("Nq,Nkv,H", [(8, 4, 64), (4, 1, 128), (3, 3, 128)])
+@pytest.mark.parametrize("sequences", [32, 33, 127, 128, 129, 200])
+def test_units_of_many_sequences(sequences, Nq, Nkv, H):
+    """Single tiles, pairs of tiles and empty sequences mixed, dealt by length or in order."""
+    lengths = [(i * i * 29 + 7 * i) % 333 if i % 5 else (i % 3) * (i % 17) for i in range(sequences)]
+    g = gen(sequences, Nq, H)
+    q, k, v = inputs(g, sum(lengths), Nq, Nkv, H)
+    cu = cu_of(lengths)
+    for causal in (True, False):
+        check(q, k, v, P().attention_packed(q, k, v, cu, causal), lengths, cu, causal)
+
+
 def test_streams_graphs_and_repetition():
     lengths = [[700, 20], [64, 1000]]
     g = gen(41)

@@ -133,3 +133,30 @@ def packed(**kw):
 def test_packed_attention_refuses(kw, rc):
     assert packed(**kw) == rc and lib().tpx_last_error()
     assert packed(T=0, q=None) == 0
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_attention_over_the_cache_wants_a_finite_scale(scale):
+    assert attend(cache(), scale=scale) == 1 and lib().tpx_last_error()
+
+
+def test_lengths_move_by_the_sequences_of_the_cache():
+    from tpp_pytorch_extension_b200._lib import TpxError
+    c = P().Int4Cache(1, 3, 1, 64, 3, 1, device="cpu")
+    for cu in ([0, 4], [0, 1, 2], [0, 1, 2, 3, 4]):
+        with pytest.raises(TpxError, match="sequences"):
+            c.advance(torch.tensor(cu, dtype=torch.int32))
+    assert c.lengths.tolist() == [0, 0, 0]
+
+
+def test_models_without_a_packed_form_say_so():
+    from tpp_pytorch_extension_b200._lib import TpxError
+    from tpp_pytorch_extension_b200.llm.fused_opt_infer import OPTRunner
+
+    class Opt(OPTRunner):
+        def __init__(self):
+            torch.nn.Module.__init__(self)
+            self.layers = [object()]
+
+    with pytest.raises(TpxError, match="packed"):
+        Opt().generate_packed([torch.zeros(3, dtype=torch.int64)], 2)

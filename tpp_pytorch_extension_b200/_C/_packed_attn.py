@@ -97,6 +97,7 @@ class Int4Cache:
 
     def advance(self, cu_seqlens=None):
         """The tokens of the call are cached: lengths grow by the sequences' tokens (by one without cu_seqlens)."""
+        _check(cu_seqlens is None or cu_seqlens.shape == (self.B + 1,), f"Int4Cache: cu_seqlens is not that of {self.B} sequences")
         self.lengths.add_(1 if cu_seqlens is None else cu_seqlens[1:] - cu_seqlens[:-1])
 
     def bytes_per_token(self):

@@ -7,7 +7,8 @@
 //
 // H / 16 lanes share a head (two pieces of 8 values per lane, which are the two halves of its rotary pairs), so that norms and ranges
 // of 64 values are a few shuffles. A warp works on heads of one kind of one token: a thread does up to UNITS of them, whose loads go out
-// together, with the products of norm weights, cosines and sines kept in registers.
+// together, with the products of norm weights, cosines and sines kept in registers. 8191 tokens, 32/8 heads of 128, norms and rotation: 45 us (3.8 TB/s,
+// 53 % of issue slots); one token: 5.4 us with the call.
 #include <numeric>
 
 #include "tpx_int4.cuh"
@@ -340,6 +341,7 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const PrepParams p) {
 // Many tokens: resident warps walk the tokens, four heads per thread. The next token's pieces and angles come by cp.async while this one is
 // worked on, each lane's into places of its own (no barrier): with loads to registers 16 warps per SM had too little in flight (8191
 // tokens, 40 heads of 128: 51 us, 3.4 TB/s).
+// Four heads: with three 52.7 us, with two 57.9 (102 with three blocks per SM), against 45.2
 constexpr int kPrepUnits = 4, kPrepWarps = 8;
 constexpr int kPrepStage = (2 * kPrepUnits + 4) * 512;  // bytes per warp: two pieces of each head, four of cosines and sines
 template <int LANES>
