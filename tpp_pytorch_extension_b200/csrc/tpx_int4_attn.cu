@@ -13,8 +13,9 @@
 //   P V  = sum over t: (p vs) (vc - 8) + p (vz + 8 vs)
 //          m16n8k16 fp16: a byte of two codes in the mantissa of 1024 is an fp16, and so is its lower code alone; both go to the matrix unit
 //          centred (one addition per pair) and the upper code's sum is the difference / 16. Centred, since p vs is rounded to fp16 and that
-//          should not be weighed with the range's offset. vs is taken relative to a power of two that follows the largest scale seen,
-//          which keeps p vs in fp16's range.
+//          should not be weighed with the range's offset. p vs is kept in units of a power of two that every row and group of 64 has for
+//          itself and that follows the largest p vs it has met: products from 2^-20 of that one up have all bits of fp16, smaller ones are
+//          off by 2^-31 of it at most, however the scales of the groups, of the tokens and of the rows' weights differ.
 // The cache is the 16-row operand: 16 tokens for keys, 16 of the head's dimensions for values. Weights get to the second product by movmatrix.
 //
 // A page of a head (4608 bytes at H = 128) is one warp's work item, fetched by cp.async into a ring of the warp's own: no barrier in the
@@ -82,6 +83,26 @@ __device__ __forceinline__ uint32_t i4_pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float i4_pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ float i4_inverse(float pow2) { return __uint_as_float(0x7f000000u - __float_as_uint(pow2)); }  // of 2^-126 .. 2^126
+// a += e b, and d = e b c, over the groups of a head: pairs of fp32 in one operation
+template <int G>
+__device__ __forceinline__ void i4_fma(float (&a)[G], float e, const float (&b)[G]) {
+  if (G == 2)
+    asm("{ .reg .b64 x, y, z;\n  mov.b64 x, {%2, %2};\n  mov.b64 y, {%3, %4};\n  mov.b64 z, {%0, %1};\n  fma.rn.f32x2 z, x, y, z;\n  mov.b64 {%0, %1}, z; }"
+        : "+f"(a[0]), "+f"(a[G - 1])
+        : "f"(e), "f"(b[0]), "f"(b[G - 1]));
+  else
+    a[0] = fmaf(e, b[0], a[0]);
+}
+template <int G>
+__device__ __forceinline__ void i4_mul(float (&d)[G], float e, const float (&b)[G], const float (&c)[G]) {
+  if (G == 2)
+    asm("{ .reg .b64 x, y, z;\n  mov.b64 x, {%2, %2};\n  mov.b64 y, {%3, %4};\n  mov.b64 z, {%5, %6};\n  mul.rn.f32x2 x, x, y;\n  mul.rn.f32x2 x, x, z;\n  mov.b64 {%0, %1}, x; }"
+        : "=f"(d[0]), "=f"(d[G - 1])
+        : "f"(e), "f"(b[0]), "f"(b[G - 1]), "f"(c[0]), "f"(c[G - 1]));
+  else
+    d[0] = e * b[0] * c[0];
+}
 __device__ __forceinline__ uint32_t i4_add_f16(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -372,7 +393,8 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
   uint2 qf[C::TILES][WPK];
   float qsc[RT], qs[RT][G];                // per row: 2^-k scale log2(e), and sums of q times scale log2(e)
   float acc[VT][G][4][4], zacc[RT][G], m_run[RT], l_run[RT];
-  int klim[RT], klim_min = 0, vexp = -126;  // values are kept in units of 2^vexp
+  float unit[RT][G];                       // acc holds sums times this power of two
+  int klim[RT], klim_min = 0;
   const int kr = (g >> 1) + 4 * (g & 1);   // row g of a 16-row tile is key kr of its first 8, row g + 8 of its last 8
 
   int stage = 0;
@@ -458,10 +480,12 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         m_run[j] = -INFINITY;
         l_run[j] = 0.0f;
 #pragma unroll
-        for (int h = 0; h < G; h++) zacc[j][h] = 0.0f;
+        for (int h = 0; h < G; h++) {
+          zacc[j][h] = 0.0f;
+          unit[j][h] = i4_pow2(126);
+        }
       }
       klim_min = p.causal ? (int)min(cap, first + now.chunk * ROWS / p.R + 1) : now.keys;
-      vexp = -126;
 #pragma unroll
       for (int v = 0; v < VT; v++)
 #pragma unroll
@@ -538,51 +562,52 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
           }
         odd = __any_sync(0xffffffffu, odd);
       }
-      // ---- the running maximum is a reference that has to follow only when a score passes it by 2^8, the unit of the values one
-      // that follows when a scale passes it by 2^7: weights times scales then stay below 2^15
+      // ---- the running maximum is a reference that has to follow only when a score passes it by 2^8, a unit when a weight times a scale
+      // may pass 2^15.9 of it: 256 + 127 + log2 of a positive float, to 0.09 below, is what its leading bits are as the mantissa of 256
       bool pass = false;
-      float top[RT];
-      uint32_t smax = 0;  // low half: the largest scale's bits
+      float top[RT], ref[RT];
+      float size[G];
+#pragma unroll
+      for (int h = 0; h < G; h++)
+        size[h] = __uint_as_float(0x43800000u | (__vmaxu2(__vmaxu2(vparam[0][0][h], vparam[0][1][h]), __vmaxu2(vparam[1][0][h], vparam[1][1][h])) & 0xffffu) << 8);
 #pragma unroll
       for (int j = 0; j < RT; j++) {
         top[j] = fmaxf(fmaxf(x[j][0][0], x[j][0][1]), fmaxf(x[j][1][0], x[j][1][1]));
-        pass |= top[j] > m_run[j] + 8.0f;
+        const float over = top[j] - m_run[j];
+        pass |= over > 8.0f;
+#pragma unroll
+        for (int h = 0; h < G; h++) pass |= over + size[h] > 2 * 383.0f + 15.8f - __uint_as_float(0x43800000u + (__float_as_uint(unit[j][h]) >> 8));
       }
-#pragma unroll
-      for (int m = 0; m < 2; m++)
-#pragma unroll
-        for (int r = 0; r < 2; r++)
-#pragma unroll
-          for (int h = 0; h < G; h++) smax = __vmaxu2(smax, vparam[m][r][h]);
-      pass |= (int)((smax >> 7) & 255) > vexp + 127 + 6;
       if (__any_sync(0xffffffffu, pass)) {
-        int e = 0;
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-          for (int r = 0; r < 2; r++)
-#pragma unroll
-            for (int h = 0; h < G; h++) {
-              const int b = (vparam[m][r][h] >> 7) & 255;
-              if (b != 255) e = max(e, b);  // not a NaN's
-            }
-        e = (int)__reduce_max_sync(0xffffffffu, (unsigned)e) - 127;
-        // the largest scale is below 2^(e + 1): with e <= vexp + 6 it stays, else it becomes 2^6 .. 2^7 units
-        const int v_new = e > vexp + 6 ? max(e - 6, -126) : vexp;
-        const float down = v_new - vexp > 126 ? 0.0f : i4_pow2(vexp - v_new);
-        vexp = v_new;
-        float alpha[RT];
+        float down[RT][G];
 #pragma unroll
         for (int j = 0; j < RT; j++) {
           float v = top[j];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-          const float m_new = fmaxf(m_run[j], v);
-          alpha[j] = m_new == m_run[j] ? 1.0f : i4_ex2(m_run[j] - m_new);
+          // a whole number: the sums change by powers of two, those of the values not at all, but for their units
+          const float m_new = fmaxf(m_run[j], ceilf(v)), d = m_new == m_run[j] ? 0.0f : m_new - m_run[j];
+          const float alpha = d <= 126.0f ? i4_pow2(-(int)d) : 0.0f, grow = i4_pow2((int)fminf(d, 126.0f)), r0 = m_new == -INFINITY ? 0.0f : m_new;
           m_run[j] = m_new;
-          l_run[j] *= alpha[j];
+          l_run[j] *= alpha;
 #pragma unroll
-          for (int h = 0; h < G; h++) zacc[j][h] *= alpha[j];
+          for (int h = 0; h < G; h++) {
+            float most = 0.0f;  // the largest weight times scale; what is not finite has no say
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+              for (int r = 0; r < 2; r++) {
+                const float w = i4_ex2(x[j][m][r] - r0) * __uint_as_float(vparam[m][r][h] << 16);
+                most = w < INFINITY ? fmaxf(most, w) : most;
+              }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            float u = d <= 126.0f ? fminf(unit[j][h] * grow, i4_pow2(126)) : i4_pow2(126);
+            if (most * u >= 32768.0f) u = i4_pow2(6 + 127 - (int)(__float_as_uint(most) >> 23));  // it becomes 2^6 .. 2^7 units
+            down[j][h] = u * alpha * i4_inverse(unit[j][h]);
+            unit[j][h] = u;
+            zacc[j][h] *= alpha;
+          }
         }
 #pragma unroll
         for (int v = 0; v < VT; v++)
@@ -591,36 +616,32 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-              for (int k = 0; k < 4; k++) acc[v][h][i][k] *= (RT == 1 ? alpha[0] : alpha[2 * v + (k & 1)]) * down;
+              for (int k = 0; k < 4; k++) acc[v][h][i][k] *= RT == 1 ? down[0][h] : down[2 * v + (k & 1)][h];
       }
-      float ref[RT];
 #pragma unroll
       for (int j = 0; j < RT; j++) ref[j] = m_run[j] == -INFINITY ? 0.0f : m_run[j];
-      const float unit = i4_pow2(min(-vexp, 126));
       // ---- weights, and values of 16 keys at a time
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         uint32_t pb[VT][RT == 1 ? 1 : G][2];
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-          float e[RT];
-#pragma unroll
-          for (int j = 0; j < RT; j++) {
-            e[j] = i4_ex2(x[j][m][r] - ref[j]);
-            l_run[j] += e[j];
-          }
-          float ps[RT][G];  // weight times scale
+          float vs[G], z[G], ps[RT][G];  // ps: weight times scale, in its unit
 #pragma unroll
           for (int h = 0; h < G; h++) {
-            const float s = __uint_as_float(vparam[m][r][h] << 16), z = fmaf(8.0f, s, __uint_as_float(vparam[m][r][h] & 0xffff0000u)), su = s * unit;
+            vs[h] = __uint_as_float(vparam[m][r][h] << 16);
+            z[h] = fmaf(8.0f, vs[h], __uint_as_float(vparam[m][r][h] & 0xffff0000u));
+          }
 #pragma unroll
-            for (int j = 0; j < RT; j++) {
-              if (odd && x[j][m][r] == -INFINITY) {  // what a row does not see leaves it alone
-                ps[j][h] = 0.0f;
-              } else {
-                ps[j][h] = e[j] * su;
-                zacc[j][h] = fmaf(e[j], z, zacc[j][h]);
-              }
+          for (int j = 0; j < RT; j++) {
+            const float e = i4_ex2(x[j][m][r] - ref[j]);
+            l_run[j] += e;
+            if (odd && x[j][m][r] == -INFINITY) {  // what a row does not see leaves it alone
+#pragma unroll
+              for (int h = 0; h < G; h++) ps[j][h] = 0.0f;
+            } else {
+              i4_mul(ps[j], e, vs, unit[j]);
+              i4_fma(zacc[j], e, z);
             }
           }
           if (RT == 1) {  // columns (row t, group): both groups' products share the operand
@@ -686,7 +707,6 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
     };
     float o[RT][G][8];
     {
-      const float up = i4_pow2(min(vexp, 126));
 #pragma unroll
       for (int j = 0; j < RT; j++) {
 #pragma unroll
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
           for (int i = 0; i < 8; i++) {
             const int c = i & 3, e = (RT == 1 ? h : j & 1) + 2 * (i >> 2);  // accumulators c odd hold 16 times their code's sum and that of c - 1
             const float sum = c & 1 ? (acc[j / 2][h][c][e] - acc[j / 2][h][c - 1][e]) * 0.0625f : acc[j / 2][h][c][e];
-            o[j][h][i] = fmaf(sum, up, zacc[j][h]);
+            o[j][h][i] = fmaf(sum, i4_inverse(unit[j][h]), zacc[j][h]);
           }
       }
     }
