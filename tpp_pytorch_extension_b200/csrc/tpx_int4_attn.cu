@@ -760,7 +760,9 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         __syncwarp();
         bool last = false;
         if (lane == 0) last = i4_arrive(p.counters + w0, word_was, p.nonce, (unsigned)(w1 - w0 + 1));
-        if (__shfl_sync(0xffffffffu, (int)last, 0)) {
+        last = __shfl_sync(0xffffffffu, (int)last, 0);
+        __syncwarp();  // orders what lane 0 has acquired before the other lanes' reads; the shuffle orders no memory
+        if (last) {
 #pragma unroll
           for (int j = 0; j < RT; j++) {
             m_run[j] = -INFINITY;
