@@ -96,9 +96,10 @@ class Int4Cache:
         self.lengths[b].zero_()
 
     def advance(self, cu_seqlens=None):
-        """The tokens of the call are cached: lengths grow by the sequences' tokens (by one without cu_seqlens)."""
+        """The tokens of the call are cached: lengths grow by the sequences' tokens. Without cu_seqlens by one, where a sequence has a page:
+        a slot that was released, or that holds nothing yet, stays at 0 while the others decode."""
         _check(cu_seqlens is None or cu_seqlens.shape == (self.B + 1,), f"Int4Cache: cu_seqlens is not that of {self.B} sequences")
-        self.lengths.add_(1 if cu_seqlens is None else cu_seqlens[1:] - cu_seqlens[:-1])
+        self.lengths.add_(self.table.amax(1) >= 0 if cu_seqlens is None else cu_seqlens[1:] - cu_seqlens[:-1])
 
     def bytes_per_token(self):
         return len(self.pools) * self.kv_heads * 36 * self.head_dim // S2
