@@ -76,6 +76,8 @@ typedef struct {
 } TpxInt4Attention;
 size_t tpx_int4_attention_scratch_bytes(int64_t T, int64_t B, int64_t Nq, int64_t kv_heads, int64_t H);
 int tpx_int4_attention(const TpxInt4Attention* a, void* stream);
+/* The same for the sequences with lengths[b] > 0 alone; rows of the others are left as they are in out. */
+int tpx_int4_attention_behind(const TpxInt4Attention* a, void* stream);
 
 /* Attention over whole prompts: softmax(q k^T * scale) v for the T rows q [T][Nq][H], k and v [T][Nkv][H] (ld* elements apart, heads
  * side by side, 16-byte aligned), each within its sequence; causal: token i of a sequence sees the keys 0 .. i. Only the rows of
@@ -90,6 +92,9 @@ typedef struct {
   int causal;
 } TpxPackedAttention;
 int tpx_packed_attention(const TpxPackedAttention* a, void* stream);
+/* The same for the sequences with lengths[b] <= 0 alone (lengths [B], int32 on the device: tokens cached before the call); rows of the
+ * others are left as they are in out. With tpx_int4_attention_behind on the same out every row of a call gets what it has to see. */
+int tpx_packed_attention_new(const TpxPackedAttention* a, const int32_t* lengths, void* stream);
 int tpx_packed_status(void* stream, unsigned* status_host);
 
 #ifdef __cplusplus

@@ -514,8 +514,9 @@ class LlamaDecoderLayer:
         cache a _packed_attn.Int4Cache with pages for the new tokens (this layer's keys and values go into it; its lengths
         stay, Int4Cache.advance() moves them after the last layer).
 
-        With cu_seqlens (int32 [B + 1]) the call holds whole prompts, the first tokens of sequences that have nothing
-        cached, and attention runs over their keys and values before they are quantized. Without it row b is the next
+        With cu_seqlens (int32 [B + 1]) sequence b has any number of new tokens: a sequence that has nothing cached attends
+        over their keys and values before they are quantized, one that has (a prompt behind an earlier turn, drafted tokens) reads
+        the cache, its new tokens included; the lengths on the device decide, sequence by sequence. Without it row b is the next
         token of sequence b, and attention reads the cache. positions (int64 [T]): rows of the rotary table, by default the
         tokens' places in their sequences. Returns [T, D]."""
         from . import _packed_attn as P
@@ -528,7 +529,11 @@ class LlamaDecoderLayer:
             ctx = P.attention_int4(q, cache, self.layer_idx)
         else:
             v = qkv[:, (self.Nq + self.Nkv) * self.H:].view(T, self.Nkv, self.H)
-            ctx = P.attention_packed(q, k, v, cu_seqlens)
+            if cache.is_new():
+                ctx = P.attention_packed(q, k, v, cu_seqlens)
+            else:
+                ctx = P.attention_packed(q, k, v, cu_seqlens, lengths=cache.lengths)
+                P.attention_int4(q, cache, self.layer_idx, cu_seqlens, out=ctx, behind=True)
         so = fc_plain_act(ctx.view(T, self.Nq * self.H), self.Wp, res=hs, res_scale=1.0 / ws)
         if ws > 1:
             allreduce(so)

@@ -29,8 +29,11 @@ class Int4Cache:
     def __init__(self, layers, pages, kv_heads, head_dim, sequences, columns, device="cuda"):
         _check(head_dim in (64, 128), f"Int4Cache: head size {head_dim} is not 64 or 128")
         _check(min(layers, pages, kv_heads, sequences, columns) > 0, "Int4Cache: sizes must be positive")
+        with torch.inference_mode(False):  # whose tensors would not count their changes
+            lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
         self._set([torch.zeros((pages, kv_heads, 36 * head_dim), dtype=torch.uint8, device=device) for _ in range(layers)],
-                  torch.full((sequences, columns), -1, dtype=torch.int32, device=device), torch.zeros(sequences, dtype=torch.int32, device=device))
+                  torch.full((sequences, columns), -1, dtype=torch.int32, device=device), lengths)
+        self._new = lengths._version
         self._held = [[] for _ in range(sequences)]
         self._free = list(range(pages - 1, -1, -1))
 
@@ -46,6 +49,7 @@ class Int4Cache:
         self._pools, self._table, self._lengths = tuple(pools), table, lengths
         self.B = table.shape[0]
         self._layers = {}
+        self._new = None
         self.layer(0)
 
     # changed in place only: the operators keep their addresses
@@ -59,6 +63,11 @@ class Int4Cache:
         if s is None:
             s = self._layers[i] = _lib.torch_ops().cache_bytes(self._pools[i], self._table, self._lengths)
         return s
+
+    def is_new(self):
+        """Whether it is certain, without a look at the device, that nothing is cached: lengths that this object has made and that nobody has written
+        to since. Not while a CUDA graph is recorded, which may be replayed later."""
+        return self._new is not None and self.lengths._version == self._new and not (self.lengths.is_cuda and torch.cuda.is_current_stream_capturing())
 
     @property
     def pages(self):
@@ -130,15 +139,18 @@ def read_int4(cache, layer, tokens, cu_seqlens=None, lengths=None):
     return _lib.torch_ops().read(cache.layer(layer), tokens, cu_seqlens, lengths)
 
 
-def attention_int4(q, cache, layer, cu_seqlens=None, causal=True, scale=None, out=None):
+def attention_int4(q, cache, layer, cu_seqlens=None, causal=True, scale=None, out=None, behind=False):
     """Attention of the call's tokens q bf16 [T, heads, head_dim] over their sequences in layer `layer` of the cache, the call's own
     keys and values (appended before) included: softmax(q k^T scale) v, bf16 like q. Token i of sequence b sees the tokens up to
-    its own place lengths[b] + i, or, with causal=False, all of its sequence. A token that sees none (no page) gives zeros."""
-    return _lib.torch_ops().int4_attention(q, cache.layer(layer), cu_seqlens, causal, scale, out)
+    its own place lengths[b] + i, or, with causal=False, all of its sequence. A token that sees none (no page) gives zeros.
+    behind=True: for the sequences alone that have tokens cached before the call; rows of the others are not written."""
+    return _lib.torch_ops().int4_attention(q, cache.layer(layer), cu_seqlens, causal, scale, out, behind)
 
 
-def attention_packed(q, k, v, cu_seqlens, causal=True, scale=None, out=None):
+def attention_packed(q, k, v, cu_seqlens, causal=True, scale=None, out=None, lengths=None):
     """Attention over whole prompts laid end to end: q bf16 [T, heads, H], k and v [T, kv_heads, H] (rows may be strided, as views of a
     q/k/v linear's output are; H 64 or 128; up to 128 heads per key head; scale > 0, H^-1/2 by default): softmax(q k^T scale) v within each sequence, where token i
-    sees the tokens 0 .. i, or with causal=False all of them. bf16 [T, heads, H]; rows of no sequence are not written."""
-    return _lib.torch_ops().packed_attention(q, k, v, cu_seqlens, causal, scale, out)
+    sees the tokens 0 .. i, or with causal=False all of them. bf16 [T, heads, H]; rows of no sequence are not written. With lengths
+    (int32 [B], the tokens cached before the call) only for the sequences that have none; rows of the others are not written: they are
+    attention_int4(..., behind=True)'s."""
+    return _lib.torch_ops().packed_attention(q, k, v, cu_seqlens, causal, scale, out, lengths)

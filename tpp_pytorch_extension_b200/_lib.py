@@ -94,7 +94,9 @@ _SIGS = {
     "tpx_int4_read": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "tpx_int4_attention_scratch_bytes": (c_sz, [c_i64] * 5),
     "tpx_int4_attention": (c_int, [c_vp, c_vp]),
+    "tpx_int4_attention_behind": (c_int, [c_vp, c_vp]),
     "tpx_packed_attention": (c_int, [c_vp, c_vp]),
+    "tpx_packed_attention_new": (c_int, [c_vp, c_vp, c_vp]),
     "tpx_packed_status": (c_int, [c_vp, ctypes.POINTER(ctypes.c_uint)]),
     "tpx_qlinear": (c_int, [c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp,
                             c_f32, c_vp, c_vp, c_sz, c_vp]),
@@ -145,8 +147,8 @@ def torch_ops():
         except ImportError as e:
             raise TpxError(f"the extension module _tpx_torch cannot be loaded ({e}): build it with `python -m tpp_pytorch_extension_b200._build`") from e
         m.bind(TpxError, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value
-                           for n in ("tpx_head_prep", "tpx_int4_read", "tpx_int4_attention_scratch_bytes", "tpx_int4_attention", "tpx_packed_attention",
-                                     "tpx_last_error")))
+                           for n in ("tpx_head_prep", "tpx_int4_read", "tpx_int4_attention_scratch_bytes", "tpx_int4_attention", "tpx_int4_attention_behind",
+                                     "tpx_packed_attention", "tpx_packed_attention_new", "tpx_last_error")))
         _torch_ops = m
     return _torch_ops
 

@@ -41,7 +41,7 @@ struct I4Params {
   unsigned long long* counters;  // [workers]
   unsigned long long nonce;      // low 16 bits zero
   int64_t ldq;
-  int T, Nq, R, causal;
+  int T, Nq, R, causal, behind;  // behind: only sequences of which tokens are cached before the call have a part in it
   float sc2;                     // scale * log2(e)
 };
 
@@ -148,6 +148,7 @@ __device__ __forceinline__ I4Seq i4_seq(const I4Params& p, int b, int rows) {
   } else {
     s.n = 1;
   }
+  if (p.behind && p.c.lengths[b] <= 0) s.n = 0;
   const long long keys = (long long)max(p.c.lengths[b], 0) + s.n, cap = (long long)p.c.cols * kI4Page;
   s.keys = (int)min(keys, cap);
   s.pages = (s.keys + kI4Page - 1) / kI4Page;
@@ -953,7 +954,7 @@ extern "C" size_t tpx_int4_attention_scratch_bytes(int64_t T, int64_t B, int64_t
   return i4_scratch(i4_rows(T, B, Nq, kv_heads), H);
 }
 
-extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
+static int int4_attention(const TpxInt4Attention* a, int behind, void* stream) {
   TPX_REQUIRE(a && a->cache && (a->T == 0 || (a->q && a->out)), TPX_ERR_ARG, "int4_attention: null pointer");
   I4Params p = {};
   const int rc = i4_cache_of(a->cache, &p.c);
@@ -983,8 +984,12 @@ extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) {
   p.Nq = (int)a->Nq;
   p.R = (int)(a->Nq / Nkv);
   p.causal = a->causal;
+  p.behind = behind;
   p.sc2 = a->scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
   if (H == 128) return rt == 1 ? i4_launch<128, 1>(p, st) : rt == 2 ? i4_launch<128, 2>(p, st) : i4_launch<128, 4>(p, st);
   return rt == 1 ? i4_launch<64, 1>(p, st) : rt == 2 ? i4_launch<64, 2>(p, st) : i4_launch<64, 4>(p, st);
 }
+
+extern "C" int tpx_int4_attention(const TpxInt4Attention* a, void* stream) { return int4_attention(a, 0, stream); }
+extern "C" int tpx_int4_attention_behind(const TpxInt4Attention* a, void* stream) { return int4_attention(a, 1, stream); }

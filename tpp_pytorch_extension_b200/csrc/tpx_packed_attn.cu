@@ -41,7 +41,7 @@ struct PkCfg {
 };
 
 struct PkParams {
-  const int32_t* cu;
+  const int32_t *cu, *cached;  // cached: sequences of which any tokens are cached have no part in the call (NULL: all have)
   const uint16_t* v;
   uint16_t* out;
   int64_t ldv;
@@ -138,6 +138,7 @@ __device__ __forceinline__ uint32_t pk_pack(float lo, float hi) {
 __device__ __forceinline__ void pk_sequence(const PkParams& p, int b, int& first, int& n) {
   first = min(max(p.cu[b], 0), p.T);
   n = max(min(max(p.cu[b + 1], 0), p.T) - first, 0);
+  if (p.cached && p.cached[b] > 0) n = 0;
 }
 // Units of a sequence. One that fills a single tile has its key heads in pairs, a tile each with keys of its own: units of one tile leave half of a
 // block idle and every step of it waiting for the one before (24 prompts of up to 300 tokens, 32 heads of 64: 42.7 us)
@@ -716,7 +717,7 @@ static int pk_launch(const TpxPackedAttention& a, PkParams& p, cudaStream_t st) 
 
 using namespace tpx;
 
-extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) {
+static int packed_attention(const TpxPackedAttention* a, const int32_t* cached, void* stream) {
   TPX_REQUIRE(a && a->cu_seqlens && (a->T == 0 || (a->q && a->k && a->v && a->out)), TPX_ERR_ARG, "packed_attention: null pointer");
   TPX_REQUIRE(a->H == 64 || a->H == 128, TPX_ERR_UNSUPPORTED, "packed_attention: head size %ld not supported (64 or 128)", (long)a->H);
   TPX_REQUIRE(a->Nkv > 0 && a->Nkv <= 1024 && a->Nq > 0 && a->Nq % a->Nkv == 0, TPX_ERR_ARG, "packed_attention: %ld query heads for %ld key heads", (long)a->Nq,
@@ -730,6 +731,7 @@ extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) {
   if (a->T == 0) return TPX_OK;
   PkParams p = {};
   p.cu = a->cu_seqlens;
+  p.cached = cached;
   p.v = a->v;
   p.out = a->out;
   p.ldv = a->ldv;
@@ -742,6 +744,13 @@ extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) {
   p.causal = a->causal;
   p.sc2 = a->scale * 1.4426950408889634f;
   return a->H == 128 ? pk_launch<128>(*a, p, (cudaStream_t)stream) : pk_launch<64>(*a, p, (cudaStream_t)stream);
+}
+
+extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) { return packed_attention(a, nullptr, stream); }
+
+extern "C" int tpx_packed_attention_new(const TpxPackedAttention* a, const int32_t* lengths, void* stream) {
+  TPX_REQUIRE(lengths, TPX_ERR_ARG, "packed_attention_new: null pointer");
+  return packed_attention(a, lengths, stream);
 }
 
 extern "C" int tpx_packed_status(void* stream, unsigned* status_host) {

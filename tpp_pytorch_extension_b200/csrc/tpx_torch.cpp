@@ -24,7 +24,9 @@ struct {
   int (*int4_read)(const TpxInt4Cache*, const int32_t*, int64_t, uint16_t*, uint16_t*, void*);
   size_t (*scratch_bytes)(int64_t, int64_t, int64_t, int64_t, int64_t);
   int (*int4_attention)(const TpxInt4Attention*, void*);
+  int (*int4_attention_behind)(const TpxInt4Attention*, void*);
   int (*packed_attention)(const TpxPackedAttention*, void*);
+  int (*packed_attention_new)(const TpxPackedAttention*, const int32_t*, void*);
   const char* (*last_error)();
 } g_lib;
 
@@ -308,9 +310,9 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   )
 }
 
-// int4_attention(q, cache, cu_seqlens, causal, scale, out) -> out
+// int4_attention(q, cache, cu_seqlens, causal, scale, out, behind) -> out
 PyObject* int4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (!arity("int4_attention", n, 6)) return nullptr;
+  if (!arity("int4_attention", n, 7)) return nullptr;
   TPX_BODY(
     Call c{"attention_int4", args};
     const at::Tensor& q = c.tensor(0, "q");
@@ -325,6 +327,7 @@ PyObject* int4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.cu_seqlens = c.cuts(2, a.cache->B, a.T);
     a.causal = c.truth(3);
     a.scale = c.none(4) ? (float)(1.0 / std::sqrt((double)H)) : (float)c.real(4);
+    const bool behind = c.truth(6);
     at::Tensor out = c.output(5, {a.T, a.Nq, H});
     a.scratch_bytes = g_lib.scratch_bytes(a.T, a.cache->B, a.Nq, Nkv, H);
     // of this call alone: calls on two streams, and two graphs, share nothing
@@ -332,14 +335,14 @@ PyObject* int4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.scratch = scratch.data_ptr();
     a.q = bf16(q);
     a.out = bf16(out);
-    c.done(g_lib.int4_attention(&a, c.stream()));
+    c.done(behind ? g_lib.int4_attention_behind(&a, c.stream()) : g_lib.int4_attention(&a, c.stream()));
     return THPVariable_Wrap(std::move(out));
   )
 }
 
-// packed_attention(q, k, v, cu_seqlens, causal, scale, out) -> out
+// packed_attention(q, k, v, cu_seqlens, causal, scale, out, lengths) -> out
 PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (!arity("packed_attention", n, 7)) return nullptr;
+  if (!arity("packed_attention", n, 8)) return nullptr;
   TPX_BODY(
     Call c{"attention_packed", args};
     const at::Tensor& q = c.tensor(0, "q"); const at::Tensor& k = c.tensor(1, "k"); const at::Tensor& v = c.tensor(2, "v");
@@ -358,22 +361,28 @@ PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a.B = THPVariable_Unpack(args[3]).size(0) - 1;
     a.causal = c.truth(4);
     a.scale = c.none(5) ? (float)(1.0 / std::sqrt((double)a.H)) : (float)c.real(5);
+    const int32_t* cached = nullptr;
+    if (!c.none(7)) {
+      const at::Tensor& l = c.tensor(7, "lengths");
+      if (l.scalar_type() != at::kInt || l.dim() != 1 || l.size(0) != a.B || !l.is_contiguous()) refuse("attention_packed: lengths must be int32 [%lld]", (long long)a.B);
+      cached = l.const_data_ptr<int32_t>();
+    }
     at::Tensor out = c.output(6, {a.T, a.Nq, a.H});
     a.q = bf16(q);
     a.k = bf16(k);
     a.v = bf16(v);
     a.out = bf16(out);
-    c.done(g_lib.packed_attention(&a, c.stream()));
+    c.done(cached ? g_lib.packed_attention_new(&a, cached, c.stream()) : g_lib.packed_attention(&a, c.stream()));
     return THPVariable_Wrap(std::move(out));
   )
 }
 
 // bind(error class, addresses of the library's functions in the order of g_lib)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (!arity("bind", n, 7)) return nullptr;
-  static_assert(sizeof(g_lib) == 6 * sizeof(void*), "addresses");
-  void* at[6];
-  for (int i = 0; i < 6; i++) {
+  if (!arity("bind", n, 9)) return nullptr;
+  static_assert(sizeof(g_lib) == 8 * sizeof(void*), "addresses");
+  void* at[8];
+  for (int i = 0; i < 8; i++) {
     at[i] = PyLong_AsVoidPtr(args[i + 1]);
     if (PyErr_Occurred()) return nullptr;
   }
