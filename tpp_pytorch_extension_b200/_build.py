@@ -4,14 +4,20 @@
 returns the whole library if that is up to date, else a library of only the sources that model needs.
 
 Every csrc/*.cu is compiled to an object under build/ (in parallel, only where the source or a header is newer than the
-object) and the objects are linked into libtpx_b200.so beside this file; csrc/tpx_torch.cpp becomes the extension module _tpx_torch.so. `TPX_DEBUG=1` in the environment adds
+object) and the objects are linked into libtpx_b200.so beside this file; csrc/tpx_torch.cpp becomes the extension module _tpx_torch.so, for the torch
+and the Python that are there. The library does without the module: where that cannot be built, a warning says so. `TPX_DEBUG=1` in the environment adds
 -DTPX_DEBUG, which compiles in the timing-experiment knobs and debug exports; the default build has none of them."""
 import concurrent.futures
+import contextlib
 import fcntl
 import glob
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SO = os.path.join(HERE, "libtpx_b200.so")
@@ -52,14 +58,41 @@ def stale(so=SO, srcs=None):
     return any(os.path.getmtime(d) > t for d in (srcs or sources()) + _headers())
 
 
+def _nvcc():
+    return os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+
+
+@contextlib.contextmanager
+def _alone():
+    """One build at a time: objects are shared."""
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(os.path.join(OBJ_DIR, "lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        yield
+
+
 def build(force=False, verbose=False, so=SO, srcs=None):
     srcs = srcs or sources()
+    if force or stale(so, srcs):
+        with _alone():
+            if force or stale(so, srcs):
+                _build_library(force, verbose, so, srcs)
     if so == SO:
-        build_torch(force)
-    if not force and not stale(so, srcs):
-        return so
-    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    os.makedirs(OBJ_DIR, exist_ok=True)
+        try:
+            if force or module_stale():
+                with _alone():
+                    if force or module_stale():
+                        _build_module()
+        except (OSError, subprocess.CalledProcessError) as e:
+            with contextlib.suppress(OSError):
+                if os.path.getmtime(TORCH_SO) < _module_sources_time():
+                    os.remove(TORCH_SO)  # it may not know the library's structures any more
+            warnings.warn(f"the extension module _tpx_torch cannot be built ({e}): the operators on packed sequences will not be there")
+    return so
+
+
+def _build_library(force, verbose, so, srcs):
+    nvcc = _nvcc()
     hdr_t = max(os.path.getmtime(h) for h in _headers())
     todo = []
     for s in srcs:
@@ -77,25 +110,58 @@ def build(force=False, verbose=False, so=SO, srcs=None):
     part = so + f".{os.getpid()}"
     subprocess.check_call([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", part] + [_obj(s) for s in srcs])
     os.replace(part, so)
-    return so
 
 
-def build_torch(force=False):
+def cuda_include():
+    """The headers beside the compiler, wherever $NVCC is found."""
+    found = shutil.which(_nvcc()) or _nvcc()
+    for nvcc in (found, os.path.realpath(found), "/usr/local/cuda/bin/nvcc"):
+        inc = os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")
+        if os.path.exists(os.path.join(inc, "cuda_runtime_api.h")):
+            return inc
+    raise FileNotFoundError(f"no CUDA headers beside {_nvcc()}")
+
+
+def _torch_dir():
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise FileNotFoundError("torch is not installed")
+    return os.path.dirname(spec.origin)
+
+
+def _made_for():
+    """What the module depends on besides its sources."""
+    with open(os.path.join(_torch_dir(), "version.py")) as f:
+        return f"{sys.version}\n{sysconfig.get_config_var('EXT_SUFFIX')}\n{f.read()}"
+
+
+def _module_sources_time():
+    return max(os.path.getmtime(f) for f in [os.path.join(HERE, "csrc", "tpx_torch.cpp")] + _headers())
+
+
+def _stamp():
+    return os.path.join(OBJ_DIR, os.path.basename(TORCH_SO) + ".made_for")
+
+
+def module_stale():
+    if not os.path.exists(TORCH_SO) or not os.path.exists(_stamp()) or os.path.getmtime(TORCH_SO) < _module_sources_time():
+        return True
+    with open(_stamp()) as f:
+        return f.read() != _made_for()
+
+
+def _build_module():
     """The extension module csrc/tpx_torch.cpp: operators on torch tensors without ctypes in between (g++, against torch's headers)."""
-    import importlib.util
-    import sysconfig
-    src = os.path.join(HERE, "csrc", "tpx_torch.cpp")
-    if not force and os.path.exists(TORCH_SO) and os.path.getmtime(TORCH_SO) >= max(os.path.getmtime(f) for f in [src] + _headers()):
-        return TORCH_SO
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
-    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    torch_dir = _torch_dir()
     inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+           sysconfig.get_paths()["include"], cuda_include()]
     part = TORCH_SO + f".{os.getpid()}"
-    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f for d in inc for f in ("-isystem", d)] + ["-o", part, src, "-L" + os.path.join(torch_dir, "lib"),
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared"] + [f for d in inc for f in ("-isystem", d)] +
+                          ["-o", part, os.path.join(HERE, "csrc", "tpx_torch.cpp"), "-L" + os.path.join(torch_dir, "lib"),
                            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], stdout=sys.stderr)
     os.replace(part, TORCH_SO)
-    return TORCH_SO
+    with open(_stamp(), "w") as f:
+        f.write(_made_for())
 
 
 def ensure(architecture):
