@@ -329,9 +329,15 @@ class LlamaRunner(torch.nn.Module):
             else:
                 step()
                 if use_graph and max_new_tokens - len(outs) > 2:  # the first step ran eagerly: scratch has its size
-                    graph = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(graph):
-                        step()
+                    try:
+                        graph = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph):
+                            step()
+                    except Exception as e:  # capture unsupported here: decode eagerly
+                        import warnings
+                        warnings.warn(f"CUDA graph capture of the decode step failed ({e!r}); decoding eagerly")
+                        graph, use_graph = None, False
+                        torch.cuda.synchronize()
             outs.append(tok.clone())
         _lib.assert_no_kernel_error()
         new = torch.cat(outs, dim=1)
