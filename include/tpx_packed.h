@@ -37,7 +37,7 @@ typedef struct {
 } TpxInt4Cache;
 
 /* One pass over the heads behind a q/k/v linear: RMS norm of every query and key head (norm weights [H], bf16 or fp32; NULL: no
- * norm), then the rotation of its first rot values in pairs (i, i + rot / 2) by the token's row of the table ep [2][max_pos][ld_ep]
+ * norm; the mean of squares in fp32, which heads with values from 2^60 on may pass), then the rotation of its first rot values in pairs (i, i + rot / 2) by the token's row of the table ep [2][max_pos][ld_ep]
  * fp32 (cosines, sines; NULL: none; positions outside [0, max_pos) leave the head as it is); q and k are rounded once, to bf16, and written to
  * q_out [T][Nq][H] and k_out [T][Nkv][H] (NULL: not written). With a cache the keys (as rounded) and the values v go to their places in it. pos NULL: a
  * token's position is its place in the cache (0 without one). H: a multiple of 16 up to 256, with a cache 64 or 128; rot a multiple of 16. Rows
@@ -61,7 +61,8 @@ int tpx_int4_read(const TpxInt4Cache* cache, const int32_t* cu_seqlens, int64_t 
 
 /* Attention over the cache: softmax(q k^T * scale) v for the T query rows q [T][Nq][H] (ldq elements apart) over the tokens of
  * their sequence in the cache, the call's own included: token i of sequence b sees the places 0 .. lengths[b] + i (causal) or all
- * of lengths[b] + n. A row that sees nothing becomes zero. scratch: tpx_int4_attention_scratch_bytes(...) bytes that nobody else
+ * of lengths[b] + n. A row that sees nothing becomes zero. Weights that differ from their row's largest by 2^126 or more are 0, weights times scales
+ * are rounded to 11 bits, or to 2^-31 of the largest such product of their row and group of 64 where that is more. scratch: tpx_int4_attention_scratch_bytes(...) bytes that nobody else
  * uses meanwhile, 256-byte aligned, of any content. */
 typedef struct {
   const uint16_t* q;

@@ -3,12 +3,14 @@
 //   y = x / sqrt(mean(x^2) + eps) * w          over the H values of a query or key head, statistics in fp32
 //   (y_i, y_i+rot/2) -> (y_i c - y_i+rot/2 s, y_i+rot/2 c + y_i s)
 // and for the cache, per 64 values of the bf16 row: code = round((x - min) / scale). One read of q/k/v, one write of q and k, 36 bytes
-// per 64 cached values: bound by HBM for prompts, by the launch and one chain of dependent loads for single tokens.
+// per 64 cached values. Single tokens are bound by the launch and one chain of dependent loads; prompts by latencies (see the counters below: neither HBM
+// nor the issue slots are full), the append by the ranges' shuffles and the codes.
 //
 // H / 16 lanes share a head (two pieces of 8 values per lane, which are the two halves of its rotary pairs), so that norms and ranges
 // of 64 values are a few shuffles. A warp works on heads of one kind of one token: a thread does up to UNITS of them, whose loads go out
-// together, with the products of norm weights, cosines and sines kept in registers. 8191 tokens, 32/8 heads of 128, norms and rotation: 45 us (3.8 TB/s,
-// 53 % of issue slots); one token: 5.4 us with the call.
+// together, with the products of norm weights, cosines and sines kept in registers. 8191 tokens, 32/8 heads of 128, norms and rotation: 45 us (3.8 TB/s
+// of inputs and outputs, HBM busy 36 %, 53 % of issue slots); one token: 5.4 us with the call. 8 key heads of 128, 32768 tokens: append alone 132 us (1.3 TB/s),
+// read-back alone 33.5 us (5.1 TB/s, HBM); 4071 tokens: 21.3 and 7.1 us.
 #include <numeric>
 
 #include "tpx_int4.cuh"
@@ -114,7 +116,11 @@ __device__ __forceinline__ void prep_to_cache(uint8_t* dst, int t, bool is_v, in
     const float base = g ? least[1] : least[0], s = g ? step[1] : step[0], y = g ? back[1] : back[0];
     uint32_t word = 0;
     if (s > 1e-30f && s < 1e30f) {
-      // The quotient with its remainder taken back in is the rounded one, as a division's would be, ties exact; 1.5 * 2^23 rounds it to a whole number
+      // v / s: the product with the reciprocal, corrected once by the remainder that a multiply-add leaves exactly (P. W. Markstein, "Computation of
+      // elementary functions on the IBM RISC System/6000 processor", IBM J. Res. Dev. 34, 1990). What codes need of it follows from s having 8
+      // bits: a quotient halfway between two codes has 5 bits and comes out as it is, since the corrected value is off by 2^-46 of itself before it is
+      // rounded; rounding is monotone, so no other quotient gets past that point. 1.5 * 2^23 then rounds it to a whole number.
+      // Where remainders might not be normal numbers: the division itself.
       float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 7; i >= 0; i--) {

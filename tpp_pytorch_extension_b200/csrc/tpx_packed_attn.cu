@@ -41,7 +41,7 @@ struct PkCfg {
 };
 
 struct PkParams {
-  const int32_t *cu, *cached;  // cached: sequences of which any tokens are cached have no part in the call (NULL: all have)
+  const int32_t *cu, *cached;  // cached: the tokens cached of each sequence, for calls of the new ones alone
   const uint16_t* v;
   uint16_t* out;
   int64_t ldv;
@@ -134,17 +134,20 @@ __device__ __forceinline__ uint32_t pk_pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Rows first .. first + n - 1 of sequence b
+// Rows first .. first + n - 1 of sequence b. PART: sequences of which tokens are cached have none (a kernel of its own: the test in the one for all
+// sequences took 543-548 us for 536-540, 8192 tokens, and 30.6 for 29.4, 24 short prompts)
+template <bool PART>
 __device__ __forceinline__ void pk_sequence(const PkParams& p, int b, int& first, int& n) {
   first = min(max(p.cu[b], 0), p.T);
   n = max(min(max(p.cu[b + 1], 0), p.T) - first, 0);
-  if (p.cached && p.cached[b] > 0) n = 0;
+  if (PART && p.cached[b] > 0) n = 0;
 }
 // Units of a sequence. One that fills a single tile has its key heads in pairs, a tile each with keys of its own: units of one tile leave half of a
 // block idle and every step of it waiting for the one before (24 prompts of up to 300 tokens, 32 heads of 64: 42.7 us)
+template <bool PART>
 __device__ __forceinline__ int pk_units(const PkParams& p, int b) {
   int first, n;
-  pk_sequence(p, b, first, n);
+  pk_sequence<PART>(p, b, first, n);
   return n <= p.TPT ? (n > 0 ? (p.Nkv + 1) / 2 : 0) : (n + 2 * p.TPT - 1) / (2 * p.TPT) * p.Nkv;
 }
 
@@ -158,8 +161,9 @@ constexpr int kPkAhead = 4;      // units that are looked up ahead
 constexpr int kPkSorted = 128;   // sequences, at most, whose units are dealt by length
 // The units of a block: rounds over all blocks, every other one backwards, since units get shorter from round to round
 __device__ __forceinline__ int pk_nth(int round) { return round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x); }
+template <bool PART>
 __device__ __forceinline__ void pk_fill(const PkParams& p, PkUnit& w, int b, bool split, int pair, int head) {
-  pk_sequence(p, b, w.tok0, w.n);
+  pk_sequence<PART>(p, b, w.tok0, w.n);
   w.split = split;
   if (split) {
     w.t0[0] = w.t0[1] = 0;
@@ -178,6 +182,7 @@ __device__ __forceinline__ void pk_fill(const PkParams& p, PkUnit& w, int b, boo
   }
 }
 // Unit u of the call, sequences in order: the last tokens (with the most keys) of a sequence first, heads of the same tokens side by side
+template <bool PART>
 __device__ __forceinline__ void pk_in_order(const PkParams& p, PkUnit& w, const int* pre, int buckets, int stride, int u) {
   int lo = 0, hi = buckets;  // pre[lo] <= u < pre[hi]
   while (hi - lo > 1) {
@@ -187,20 +192,21 @@ __device__ __forceinline__ void pk_in_order(const PkParams& p, PkUnit& w, const 
   }
   int at = pre[lo], b = lo * stride, units = 0;
   for (; b < p.B; b++) {
-    units = pk_units(p, b);
+    units = pk_units<PART>(p, b);
     if (u < at + units) break;
     at += units;
   }
   b = min(b, p.B - 1);
   int first, n;
-  pk_sequence(p, b, first, n);
+  pk_sequence<PART>(p, b, first, n);
   const int k = u - at;
-  if (n <= p.TPT) pk_fill(p, w, b, true, 0, k);
-  else pk_fill(p, w, b, false, units / p.Nkv - 1 - k / p.Nkv, k % p.Nkv);
+  if (n <= p.TPT) pk_fill<PART>(p, w, b, true, 0, k);
+  else pk_fill<PART>(p, w, b, false, units / p.Nkv - 1 - k / p.Nkv, k % p.Nkv);
 }
 // Unit u of the call, those with the most keys first: pair by pair of tiles from the end of the longest sequence down, the pairs of all sequences that
 // are as long side by side, sequences of a single tile last. A warp looks one up together: pairs[i] are those of its sequence 32 i + lane, 0 in a
 // single tile (single: such a sequence). Units in order of the sequences: 16 prompts of up to 2048 tokens 85.3 us
+template <bool PART>
 __device__ __forceinline__ void pk_by_length(const PkParams& p, PkUnit& w, const int (&pairs)[kPkSorted / 32], const unsigned (&single)[kPkSorted / 32], int most, int u) {
   auto above = [&](int k) {  // units of pairs k and later
     int v = 0;
@@ -229,10 +235,10 @@ __device__ __forceinline__ void pk_by_length(const PkParams& p, PkUnit& w, const
     if (b < 0 && m < n) b = 32 * i + __fns(has, 0, m + 1);
     m -= n;
   }
-  pk_fill(p, w, max(b, 0), !in_pairs, lo, r % each);
+  pk_fill<PART>(p, w, max(b, 0), !in_pairs, lo, r % each);
 }
 
-template <int H>
+template <int H, bool PART>
 __global__ void __launch_bounds__(kPkThreads, 1)
 packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const PkParams p) {
@@ -283,7 +289,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
   {
     const int per = (buckets + kPkThreads - 1) / kPkThreads, lo = min((int)threadIdx.x * per, buckets), hi = min(lo + per, buckets);
     int mine = 0;
-    for (int b = lo * stride; b < min(hi * stride, p.B); b++) mine += pk_units(p, b);
+    for (int b = lo * stride; b < min(hi * stride, p.B); b++) mine += pk_units<PART>(p, b);
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -300,7 +306,7 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
     for (int k = lo; k < hi; k++) {
       pre[k] = at;
-      for (int b = k * stride; b < min((k + 1) * stride, p.B); b++) at += pk_units(p, b);
+      for (int b = k * stride; b < min((k + 1) * stride, p.B); b++) at += pk_units<PART>(p, b);
     }
     if (threadIdx.x == 0) pre[buckets] = total;
   }
@@ -455,13 +461,16 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------ units, ahead of those who work on them
+    // By length, as long as a warp can hold the sizes of all sequences: 16 prompts of up to 2048 72.5 us, in order of the sequences 84.4; 120 of up to 1000
+    // 283 and 308; 200, with twice the table, 508-532 and 543. Not causal, every pair of a sequence takes all of its keys, and the order of the
+    // sequences is the faster one for many: 200 prompts 807 us by length, 722 in order (16: 120 and 118)
     const bool sorted = p.causal && p.B <= kPkSorted;
     int pairs[kPkSorted / 32], most = 0;
     unsigned single[kPkSorted / 32];
 #pragma unroll
     for (int i = 0; i < kPkSorted / 32; i++) {
       int first, n = 0;
-      if (sorted && 32 * i + lane < p.B) pk_sequence(p, 32 * i + lane, first, n);
+      if (sorted && 32 * i + lane < p.B) pk_sequence<PART>(p, 32 * i + lane, first, n);
       pairs[i] = n <= p.TPT ? 0 : (n + 2 * p.TPT - 1) / (2 * p.TPT);
       single[i] = __ballot_sync(0xffffffffu, n > 0 && n <= p.TPT);
       most = max(most, pairs[i]);
@@ -475,8 +484,8 @@ packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         break;
       }
       PkUnit w;
-      if (sorted) pk_by_length(p, w, pairs, single, most, u);
-      else pk_in_order(p, w, pre, buckets, stride, u);
+      if (sorted) pk_by_length<PART>(p, w, pairs, single, most, u);
+      else pk_in_order<PART>(p, w, pre, buckets, stride, u);
       if (lane == 0) {
         ring[slot] = w;
         tc_mbar_arrive(tc_smem_u32(&u_full[slot]));
@@ -691,7 +700,7 @@ static int pk_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* 
   return TPX_OK;
 }
 
-template <int H>
+template <int H, bool PART>
 static int pk_launch(const TpxPackedAttention& a, PkParams& p, cudaStream_t st) {
   using C = PkCfg<H>;
   CUtensorMap mq, mk, mv;
@@ -705,11 +714,11 @@ static int pk_launch(const TpxPackedAttention& a, PkParams& p, cudaStream_t st) 
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 16 || !opted[dev]) {
-    TPX_CUDA_OK(cudaFuncSetAttribute(packed_attn_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    TPX_CUDA_OK(cudaFuncSetAttribute(packed_attn_kernel<H, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
     if (dev >= 0 && dev < 16) opted[dev] = true;
   }
   const int64_t most = ((int64_t)p.T / (2 * p.TPT) + p.B) * p.Nkv;  // units at most, whatever the lengths
-  TPX_CUDA_OK(launch_pdl(packed_attn_kernel<H>, dim3((unsigned)(most < sm_count() ? most : sm_count())), dim3(kPkThreads), C::SMEM, st, mq, mk, mv, p));
+  TPX_CUDA_OK(launch_pdl(packed_attn_kernel<H, PART>, dim3((unsigned)(most < sm_count() ? most : sm_count())), dim3(kPkThreads), C::SMEM, st, mq, mk, mv, p));
   return TPX_OK;
 }
 
@@ -743,7 +752,9 @@ static int packed_attention(const TpxPackedAttention* a, const int32_t* cached, 
   p.TPT = 128 / p.R;
   p.causal = a->causal;
   p.sc2 = a->scale * 1.4426950408889634f;
-  return a->H == 128 ? pk_launch<128>(*a, p, (cudaStream_t)stream) : pk_launch<64>(*a, p, (cudaStream_t)stream);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (cached) return a->H == 128 ? pk_launch<128, true>(*a, p, st) : pk_launch<64, true>(*a, p, st);
+  return a->H == 128 ? pk_launch<128, false>(*a, p, st) : pk_launch<64, false>(*a, p, st);
 }
 
 extern "C" int tpx_packed_attention(const TpxPackedAttention* a, void* stream) { return packed_attention(a, nullptr, stream); }
