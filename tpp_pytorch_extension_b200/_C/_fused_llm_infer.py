@@ -516,7 +516,8 @@ class LlamaDecoderLayer:
 
         With cu_seqlens (int32 [B + 1]) sequence b has any number of new tokens: a sequence that has nothing cached attends
         over their keys and values before they are quantized, one that has (a prompt behind an earlier turn, drafted tokens) reads
-        the cache, its new tokens included; the lengths on the device decide, sequence by sequence. Without it row b is the next
+        the cache, its new tokens included; the lengths on the device decide, sequence by sequence (both attentions are called, and
+        the limits of both hold, unless Int4Cache.is_new()). Without it row b is the next
         token of sequence b, and attention reads the cache. positions (int64 [T]): rows of the rotary table, by default the
         tokens' places in their sequences. Returns [T, D]."""
         from . import _packed_attn as P

@@ -24,8 +24,8 @@
 // on the device. A segment that is cut leaves partial results in scratch, which the group that finishes it last adds up in the order of
 // the pieces: results do not depend on who is last. Arrivals are counted in words that carry the call's own number, so that scratch may
 // hold anything before, and calls share none.
-// One sequence of 131072 tokens, 32/8 heads of 128: 44 us, of which 12 are the launch's start and end (1024 tokens: 12.5 us) and the rest pages
-// at 4.8 TB/s, 55 % of issue slots. 16 of 2048: 19.9 us; 64 of up to 4096 with 64/8 heads: 34.8 us; 8 times 5 tokens over up to 1500, 32/32 heads of 64: 15.7 us.
+// One sequence of 131072 tokens, 32/8 heads of 128: 42.9 us, of which 12 are the launch's start and end (1024 tokens: 12.4 us; a launch without work: 4.4) and the rest
+// pages at 4.9 TB/s, 55 % of issue slots. 16 of 2048: 19.4 us; 64 of up to 4096 with 64/8 heads: 35.5 us; 8 times 5 tokens over up to 1500, 32/32 heads of 64: 15.8 us.
 #include "tpx_int4.cuh"
 
 namespace tpx {
@@ -567,7 +567,8 @@ __global__ void __launch_bounds__(I4Cfg<H, RT>::WARPS * 32, 1) int4_attn_kernel(
         odd = __any_sync(0xffffffffu, odd);
       }
       // ---- the running maximum is a reference that has to follow only when a score passes it by 2^8, a unit when a weight times a scale
-      // may pass 2^15.9 of it: 256 + 127 + log2 of a positive float, to 0.09 below, is what its leading bits are as the mantissa of 256
+      // may pass 2^15.9 of it: the leading bits of a positive float, as the mantissa of 256, are 256 + 127 + its log2, to 0.09 below. (The products
+      // themselves, once rounded, as the test: 46.4 us for 44.0, 131072 tokens)
       bool pass = false;
       float top[RT], ref[RT];
       float size[G];
