@@ -62,7 +62,8 @@ int tpx_int4_read(const TpxInt4Cache* cache, const int32_t* cu_seqlens, int64_t 
 /* Attention over the cache: softmax(q k^T * scale) v for the T query rows q [T][Nq][H] (ldq elements apart) over the tokens of
  * their sequence in the cache, the call's own included: token i of sequence b sees the places 0 .. lengths[b] + i (causal) or all
  * of lengths[b] + n. A row that sees nothing becomes zero. Weights that differ from their row's largest by 2^126 or more are 0, weights times scales
- * are rounded to 11 bits, or to 2^-31 of the largest such product of their row and group of 64 where that is more. scratch: tpx_int4_attention_scratch_bytes(...) bytes that nobody else
+ * are rounded to 11 bits, or to 2^-31 of the largest such product of their row and group of 64 where that is more. Sums are fp32, of weights up to 2^8
+ * before they are divided: values from 2^100 on may pass them (here and in tpx_packed_attention). scratch: tpx_int4_attention_scratch_bytes(...) bytes that nobody else
  * uses meanwhile, 256-byte aligned, of any content. */
 typedef struct {
   const uint16_t* q;

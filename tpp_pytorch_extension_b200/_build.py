@@ -115,7 +115,7 @@ def _build_library(force, verbose, so, srcs):
 def cuda_include():
     """The headers beside the compiler, wherever $NVCC is found."""
     found = shutil.which(_nvcc()) or _nvcc()
-    for nvcc in (found, os.path.realpath(found), "/usr/local/cuda/bin/nvcc"):
+    for nvcc in (os.path.abspath(found), os.path.realpath(found), "/usr/local/cuda/bin/nvcc"):
         inc = os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include")
         if os.path.exists(os.path.join(inc, "cuda_runtime_api.h")):
             return inc
