@@ -14,7 +14,7 @@
 // passes it by 2^8: the row's O and sum are then rescaled by the softmax thread itself (O is complete up to the tile before whenever
 // scores arrive, since commits cover all earlier MMAs). P is rounded to bf16 for the MMA, the row sum adds the unrounded weights.
 //
-// 8192 tokens, 32/8 heads of 128: 535-543 us, 1.01-1.03 PFLOP/s. The tensor pipe is busy 60 % of the time, the exponentials 57 %; instructions are what the
+// 8192 tokens, 32/8 heads of 128: 535-549 us, 1.00-1.03 PFLOP/s. The tensor pipe is busy 60 % of the time, the exponentials 57 %; instructions are what the
 // loop is short of next (issue slots 32 %, but from code that does not stay in the nearest instruction cache), so less code per step is faster code. 16
 // prompts of up to 2048: 75 us; 24 of up to 300, 32/32 heads of 64: 29 us, where each unit is one chain of dependent steps.
 //
